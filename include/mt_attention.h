@@ -246,6 +246,61 @@ int mt_gqa_attn_decode_append(const void* q, const void* k, const void* v, const
                               float scale, int in_dtype, int dtype, void* workspace, size_t workspace_bytes,
                               void* stream);
 
+/*
+ * Generation over a tree of drafted tokens (no reference counterpart: its
+ * generate, src/mega_trading/model.py:134-147, makes one token a pass).  Every
+ * sequence has N <= 64 nodes behind its `length` cached tokens.  parents [B, N]
+ * int32 (rows parents_stride apart, 0: one tree for all): an earlier node, or -1
+ * for a root.  Any other parent, and any node below such a one, is padding: its
+ * rows of the results are zeros and no node sees it.  length_dev, when not NULL,
+ * holds the cached lengths (int32) in device memory, read when the kernels run and
+ * clamped to [0, capacity]: one for all (length_stride 0) or one a sequence (1);
+ * else `length` is that of all.
+ *
+ * mt_tree_rope: q [B,Hq,N,D] and k [B,Hkv,N,D] (strides: 8 int64 = q, k in (b, h, n, d)
+ * order; bf16, fp16 or fp32; D a multiple of 8) rotated by position length + depth,
+ * depth = the number of a node's ancestors, with row min(position, table_rows - 1)
+ * of the fp32 tables [table_rows, D/2]; q_out and k_out contiguous.  fp32
+ * arithmetic, one rounding.
+ */
+int mt_tree_rope(const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides, const float* rope_cos,
+                 const float* rope_sin, int table_rows, const int* parents, int64_t parents_stride,
+                 const int* length_dev, int length_stride, int length, int B, int Hq, int Hkv, int N, int D, int dtype,
+                 void* stream);
+
+/*
+ * Attention of the nodes (rotated, if RoPE is used) over the cached prefix, their
+ * ancestors and themselves: o[n] = softmax(scale q[n] . keys) values over the keys
+ * 0 .. length-1 of the caches and the k, v rows of n and its ancestors.  q
+ * [B,Hq,N,D], k/v [B,Hkv,N,D], caches [B,Hkv,capacity,D] (capacity 0: none), o
+ * contiguous [B,Hq,N,D].  strides: 20 int64 = q, k, v, k_cache, v_cache in
+ * (b, h, n or t, d) order.  Any group size Hq / Hkv; bf16 or fp16; D 32, 64 or 128.
+ * The scores and sums are fp32, the probabilities rounded to 16 bits for the
+ * product with the values.  Keys and values of padding are not used, whatever they
+ * hold.  workspace: 16-byte aligned, mt_tree_attn_workspace_size bytes with keys =
+ * capacity when length_dev is given, else length (may be NULL when that is 0).
+ */
+size_t mt_tree_attn_workspace_size(int B, int Hq, int Hkv, int N, int keys, int D);
+int mt_tree_attn(const void* q, const void* k, const void* v, const void* k_cache, const void* v_cache, void* o,
+                 const int64_t* strides, const int* parents, int64_t parents_stride, const int* length_dev,
+                 int length_stride, int length, int capacity, int B, int Hq, int Hkv, int N, int D, float scale,
+                 int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The accepted nodes into the caches of every layer: for j < count[b],
+ *   key_caches[l][b, :, length + j] = keys[l][b, :, path[b, j]],  values alike.
+ * keys / values / key_caches / value_caches: host arrays of `layers` device
+ * pointers; strides: 16 int64 = keys, values, key_caches, value_caches in
+ * (b, h, n or t, d) order, one set for all layers.  path [B, N] int32 contiguous,
+ * count [B] int32 (as mt_topk_verify writes them).  Nodes outside [0, N) and
+ * positions at or past the capacity are skipped.  16-bit types; a launch for every 32
+ * layers.  The nodes' rows must not overlap the caches.
+ */
+int mt_tree_commit(const void* const* keys, const void* const* values, void* const* key_caches,
+                   void* const* value_caches, int layers, const int64_t* strides, const int* path, const int* count,
+                   const int* length_dev, int length_stride, int length, int capacity, int B, int Hkv, int N, int D,
+                   int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

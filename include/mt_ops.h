@@ -218,6 +218,58 @@ int mt_linear_rows_gate(const void* x, int64_t x_row_stride, const void* w_gate,
 int mt_topk_sample(const void* logits, int64_t row_stride, const void* noise, int64_t noise_row_stride, int rows,
                    int vocab, int k, int64_t* tokens, int dtype, void* stream);
 
+/* Verification of a tree of drafted tokens against the target's probabilities
+ * from given random numbers, and the draw after it.  Sequence b has `nodes` <= 64
+ * nodes: node n's token is tokens[b, n] (int64), its parent parents[b, n] (int32;
+ * an earlier node, or -1 for node 0; rows parents_stride apart, 0 for one tree for
+ * all).  Row n of `logits` [B, nodes, vocab] holds the target's logits after node
+ * n, row n of `draft_logits` (or NULL) those that n's children were drawn from.
+ * strides: 4 int64 = (b, n) of logits and of draft_logits; the last stride is 1.
+ *
+ * The walk starts at node 0, the last token already accepted (its token is not
+ * read).  At node u: p = softmax over the logits of u that are >= their k-th
+ * largest (ties kept, as mt_topk_sample), q the same of draft_logits.  u's
+ * children in index order, child c with token x: if uniform[b, c] * q(x) < p(x)
+ * the walk goes on from c; else p becomes max(p - q, 0) scaled to sum 1 (p stays
+ * where that is zero everywhere).  Without draft_logits q is 1 at x and 0
+ * elsewhere.  When no child is left, token[b] = the first index of the largest
+ * p / noise[b] (Exponential(1) noise).  With uniform numbers in [0, 1) and children
+ * drawn from q (or picked without regard to chance) the tokens are distributed as
+ * the target's own top-k draws.  NaN and -inf logits count as the lowest fp32
+ * value, +inf as the highest; a token outside the vocabulary is never accepted.
+ *
+ * path [B, nodes] int32: the accepted nodes in order, node 0 first, then -1;
+ * count [B] int32: how many.  Any other parent makes a node padding, which is not
+ * visited, nor is what hangs below it; a sequence whose node 0 is padding has
+ * count 0 and token 0.  tokens, uniform and path are contiguous.  dtype: of both
+ * logits, any of the three.  1 <= vocab <= 32768, 1 <= k <= vocab, B >= 0.
+ * workspace: 16-byte aligned, mt_topk_verify_workspace_size bytes (draft: nonzero
+ * with draft_logits).  fp32 arithmetic. */
+size_t mt_topk_verify_workspace_size(int B, int nodes, int vocab, int k, int draft);
+int mt_topk_verify(const void* logits, const void* draft_logits, const int64_t* strides, const int64_t* tokens,
+                   const int* parents, int64_t parents_stride, const float* uniform, const float* noise,
+                   int64_t noise_row_stride, int* path, int* count, int64_t* token, int B, int nodes, int vocab, int k,
+                   int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Distillation from a teacher's top logits.  Row r of logits [rows, vocab] (row
+ * stride row_stride >= vocab, any alignment of its type) has `entries` <= 1024
+ * teacher logits (fp32) with their vocabulary indices (int64), both contiguous
+ * [rows, entries].  An index below 0 or a teacher logit of -inf is no entry; a row
+ * without entries counts nothing.  With T = temperature > 0,
+ *   p = softmax(teacher / T) over the row's entries,
+ *   *loss = T^2 / n sum_r sum_j p_j (log p_j - log softmax(logits / T)[index_j]),
+ * n = *count = the rows with entries (0 of them: loss 0).  An index >= vocab makes
+ * its row NaN.  fp32 arithmetic, the rows summed in 64 bits in a fixed order.
+ * row_state [rows, 4] fp32, 16-byte aligned, is written for the backward:
+ *   dlogits = *grad T / n (softmax(logits / T) - P),  P[v] = sum of p_j with index_j = v,
+ * contiguous [rows, vocab] in dtype, zero in rows without entries. */
+int mt_topk_distill_fwd(const void* logits, int64_t row_stride, const float* teacher, const int64_t* index,
+                        int64_t rows, int vocab, int entries, float temperature, float* row_state, float* loss,
+                        float* count, int dtype, void* stream);
+int mt_topk_distill_bwd(const void* logits, int64_t row_stride, const float* teacher, const int64_t* index,
+                        const float* row_state, const float* count, const float* grad, void* dlogits, int64_t rows,
+                        int vocab, int entries, float temperature, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

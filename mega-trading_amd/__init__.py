@@ -10,6 +10,8 @@ name carries a hyphen).  Public API:
 * ``attention_forward(...)`` -- forward returning ``(output, logsumexp)``.
 * ``decode_attention(query, key_cache, value_cache, length, *, repeats)`` --
   one new token against a KV cache (KV-cached ``generate``).
+* ``tree_rope``, ``tree_attention``, ``tree_commit`` -- the same for a tree of
+  drafted tokens per sequence, with ``ops.topk_verify`` between them.
 * ``rms_norm``, ``add_rms_norm``, ``swiglu_gate`` -- the decoder's
   memory-bound operators (``triton_ops.py:11-61``) on HIP kernels (``ops``).
 * ``model`` -- the Llama-style order-flow decoder that calls them
@@ -18,11 +20,12 @@ name carries a hyphen).  Public API:
 """
 
 from . import _native, model, ops, workload
-from .attention import SUPPORTED_HEAD_DIMS, attention, attention_forward, decode_attention, rope_attention
+from .attention import (SUPPORTED_HEAD_DIMS, attention, attention_forward, decode_attention, rope_attention, tree_attention,
+                        tree_commit, tree_rope)
 from .ops import add_rms_norm, rms_norm, swiglu_gate
 
 __all__ = ["attention", "rope_attention", "attention_forward", "decode_attention", "SUPPORTED_HEAD_DIMS",
-           "rms_norm", "add_rms_norm",
+           "tree_rope", "tree_attention", "tree_commit", "rms_norm", "add_rms_norm",
            "swiglu_gate", "model", "ops", "workload"]
 
 # The ops' GPU kernels and autograd are in the library: a program that calls the

@@ -61,6 +61,14 @@ EXPORTS = (
     "mt_linear_rows",
     "mt_linear_rows_gate",
     "mt_topk_sample",
+    "mt_tree_rope",
+    "mt_tree_attn_workspace_size",
+    "mt_tree_attn",
+    "mt_tree_commit",
+    "mt_topk_verify_workspace_size",
+    "mt_topk_verify",
+    "mt_topk_distill_fwd",
+    "mt_topk_distill_bwd",
 )
 
 _lock = threading.Lock()
@@ -104,6 +112,14 @@ _OPS_SIGNATURES = {
     "mt_linear_rows": (_I, [_P, _L, _P, _P, _P, _I, _P, _L, _I, _I, _I, _P]),
     "mt_linear_rows_gate": (_I, [_P, _L, _P, _P, _L, _L, _P, _L, _I, _I, _I, _I, _P]),
     "mt_topk_sample": (_I, [_P, _L, _P, _L, _I, _I, _I, _P, _I, _P]),
+    "mt_tree_rope": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _P, _L, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "mt_tree_attn_workspace_size": (_S, [_I, _I, _I, _I, _I, _I]),
+    "mt_tree_attn": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _L, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _S, _P]),
+    "mt_tree_commit": (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "mt_topk_verify_workspace_size": (_S, [_I, _I, _I, _I, _I]),
+    "mt_topk_verify": (_I, [_P, _P, _P, _P, _P, _L, _P, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _P, _S, _P]),
+    "mt_topk_distill_fwd": (_I, [_P, _L, _P, _P, _L, _I, _I, _F, _P, _P, _P, _I, _P]),
+    "mt_topk_distill_bwd": (_I, [_P, _L, _P, _P, _P, _P, _P, _P, _L, _I, _I, _F, _I, _P]),
 }
 
 

@@ -29,10 +29,14 @@ import torch
 from . import _native
 
 __all__ = ["attention", "rope_attention", "rope_attention_packed", "attention_forward", "decode_attention",
-           "SUPPORTED_HEAD_DIMS", "KERNEL_HEAD_DIMS", "MAX_HEAD_DIM", "MAX_DECODE_REPEATS"]
+           "tree_rope", "tree_attention", "tree_commit",
+           "SUPPORTED_HEAD_DIMS", "KERNEL_HEAD_DIMS", "MAX_HEAD_DIM", "MAX_DECODE_REPEATS", "MAX_TREE_NODES"]
 
 # query heads per KV head one decode launch serves; larger groups run as several launches
 MAX_DECODE_REPEATS = 8
+
+# nodes of one drafted tree (a node's ancestors are one 64-bit word)
+MAX_TREE_NODES = 64
 
 # head sizes the kernels are built for; any other head_dim up to MAX_HEAD_DIM is
 # zero-padded to the next one (the reference's forward takes any D, rounding its
@@ -293,6 +297,159 @@ def decode_append_attention(query: torch.Tensor, key: torch.Tensor, value: torch
 
 
 # ---------------------------------------------------------------------------
+# a tree of drafted tokens behind the cache (inference only)
+# ---------------------------------------------------------------------------
+def tree_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, length,
+              parents: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """RoPE of a drafted tree's nodes: ``(rot(query), rot(key))``, contiguous.
+
+    ``query`` [B, Hq, N, D], ``key`` [B, Hkv, N, D] (bf16, fp16 or fp32; D a
+    multiple of 8) hold the N <= 64 nodes of every sequence's tree.  ``parents``
+    int32 [N] (one tree for all) or [B, N]: an earlier node, or -1 for a root, the
+    nodes right behind the cached tokens.  Node n is rotated by position ``length``
+    + depth(n), the number of its ancestors.  Any other parent, -2 say, makes a
+    node padding, as does a padding ancestor; padding comes back as zeros.
+
+    ``length``: the cached tokens, an int, or an int32 GPU tensor of one element or
+    one per sequence, read when the kernel runs.  ``cos`` / ``sin`` are the
+    RotaryEmbedding tables; positions past their last row take that row, so keep
+    ``length`` plus the tree's depth within them."""
+    _check_nodes(query, key, key, (torch.float16, torch.bfloat16, torch.float32))
+    b, _, n, d = query.shape
+    if d % 8:
+        raise ValueError(f"tree_rope needs a head_dim that is a multiple of 8 (got {d})")
+    for name, tab in (("cos", cos), ("sin", sin)):
+        if tab.shape[-1] != d // 2 or not tab.is_floating_point():
+            raise ValueError(f"RoPE {name} table must be floating point with last dimension head_dim/2 = {d // 2}")
+        if tab.device != query.device:
+            raise RuntimeError(f"RoPE {name} table must be on the device of query")
+    rows = min(cos.numel(), sin.numel()) // (d // 2)
+    if rows < 1:
+        raise ValueError("the RoPE tables must have rows")
+    length_dev, length = _check_tree(parents, length, b, n, rows - 1, query.device)
+    _native.ensure()
+    return _tree_rope(query, key, cos, sin, length_dev, length, parents)
+
+
+def tree_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
+                   value_cache: torch.Tensor, length, parents: torch.Tensor, *, repeats: int) -> torch.Tensor:
+    """Attention of a drafted tree's nodes against a KV cache: node n attends to
+    the ``length`` cached tokens, its ancestors and itself.
+
+    ``query`` [B, Hq, N, D] and ``key`` / ``value`` [B, Hkv, N, D] are the nodes'
+    (rotated, see ``tree_rope``, where the caches are), ``key_cache`` /
+    ``value_cache`` [B, Hkv, capacity, D] the cached tokens' (a capacity of 0 is
+    none); 16-bit, head_dim 32, 64 or 128, Hq = Hkv * ``repeats`` for any
+    ``repeats``.  ``parents`` and ``length`` as for ``tree_rope``; a tensor
+    ``length`` is clamped to [0, capacity], and the launch then covers the whole
+    capacity and can be recorded in a HIP graph.  Returns [B, Hq, N, D],
+    contiguous; zeros at padding, whose keys and values are not used.
+
+    A chain of one node is ``decode_attention`` with the new token's key and value
+    outside the cache.  The caches are not written: ``tree_commit`` writes the
+    nodes that the verification (``ops.topk_verify``) accepts."""
+    _check_nodes(query, key, value, tuple(_KERNEL_DTYPES))
+    b, hq, n, d = query.shape
+    if key.shape[1] * repeats != hq:
+        raise ValueError("query heads must equal key/value heads multiplied by repeats")
+    if d not in KERNEL_HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {KERNEL_HEAD_DIMS} (got {d})")
+    _check_caches((key_cache,), (value_cache,), key)
+    length_dev, length = _check_tree(parents, length, b, n, key_cache.shape[2], query.device)
+    _native.ensure()
+    return _tree_attn(query, key, value, key_cache, value_cache, length_dev, length, parents, 1.0 / math.sqrt(d))
+
+
+def tree_commit(keys, values, path: torch.Tensor, count: torch.Tensor, length, key_caches, value_caches) -> None:
+    """The accepted nodes of a drafted tree into the KV caches of every layer:
+    ``key_caches[l][b, :, length + j] = keys[l][b, :, path[b, j]]`` for
+    ``j < count[b]``, and the same for the values.
+
+    ``keys`` / ``values``: one [B, Hkv, N, D] tensor per layer, as that layer's
+    ``tree_attention`` took them; ``key_caches`` / ``value_caches``: one
+    [B, Hkv, capacity, D] tensor per layer, written in place (unit last stride).
+    ``path`` [B, N] and ``count`` [B] int32 as ``ops.topk_verify`` returns them,
+    ``length`` as for ``tree_attention``: the cached tokens before this call, which
+    are ``length + count`` after it.  Nodes outside the tree and positions at or
+    past the capacity are skipped.  One launch for every 32 layers of one layout."""
+    keys, values, key_caches, value_caches = (list(x) for x in (keys, values, key_caches, value_caches))
+    if not keys or not len(keys) == len(values) == len(key_caches) == len(value_caches):
+        raise ValueError("keys, values, key_caches and value_caches must hold one tensor per layer, at least one")
+    first = keys[0]
+    _check_nodes(first, first, first, tuple(_KERNEL_DTYPES))
+    for t in (*keys, *values):
+        if t.shape != first.shape:
+            raise ValueError("keys and values must share one shape [batch, heads, nodes, head_dim]")
+        if t.dtype != first.dtype or t.device != first.device:
+            raise RuntimeError("keys and values must share one dtype and device")
+    _check_caches(key_caches, value_caches, first)
+    for t in (*key_caches, *value_caches):
+        if t.shape != key_caches[0].shape:
+            raise ValueError("the caches must share one shape")
+        if t.stride(-1) != 1:
+            raise ValueError("the caches must have a unit last-dim stride")
+    b, _, n, _ = first.shape
+    for name, t, shape in (("path", path, (b, n)), ("count", count, (b,))):
+        if t.dtype != torch.int32 or tuple(t.shape) != shape:
+            raise ValueError(f"{name} must be int32 of shape {list(shape)} (got {t.dtype}, {list(t.shape)})")
+        if t.device != first.device:
+            raise RuntimeError(f"{name} must be on the device of the keys")
+    length_dev, length = _check_length(length, b, key_caches[0].shape[2], first.device)
+    _native.ensure()
+    _tree_commit(keys, values, path, count, length_dev, length, key_caches, value_caches)
+
+
+def _check_nodes(query, key, value, dtypes) -> None:
+    if query.device.type != "cuda":
+        raise RuntimeError("hip attention backend requires ROCm GPU tensors")
+    if query.dtype not in dtypes:
+        raise RuntimeError("unsupported dtype %s (%s)" % (query.dtype, ", ".join(str(t) for t in dtypes)))
+    if query.ndim != 4 or key.ndim != 4 or value.ndim != 4:
+        raise ValueError("query, key and value must be [batch, heads, nodes, head_dim]")
+    if key.shape != value.shape:
+        raise ValueError("key and value must have the same shape")
+    if key.shape[0] != query.shape[0] or key.shape[2:] != query.shape[2:]:
+        raise ValueError("query, key and value must agree on batch, nodes and head_dim")
+    if key.shape[1] < 1 or query.shape[1] % key.shape[1] or query.shape[1] < 1:
+        raise ValueError("query heads must be a positive multiple of the key/value heads")
+    if query.shape[0] < 1 or not 1 <= query.shape[2] <= MAX_TREE_NODES:
+        raise ValueError(f"need a batch and 1 to {MAX_TREE_NODES} nodes (got {query.shape[0]}, {query.shape[2]})")
+    for t in (key, value):
+        if t.dtype != query.dtype or t.device != query.device:
+            raise RuntimeError("query, key and value must share one dtype and device")
+
+
+def _check_caches(key_caches, value_caches, key) -> None:
+    for kc, vc in zip(key_caches, value_caches):
+        if kc.ndim != 4 or kc.shape != vc.shape:
+            raise ValueError("key and value caches must have the same shape [batch, heads, capacity, head_dim]")
+        if kc.shape[:2] != key.shape[:2] or kc.shape[3] != key.shape[3]:
+            raise ValueError("the caches must have the batch, heads and head_dim of the nodes' keys")
+        for t in (kc, vc):
+            if t.dtype != key.dtype or t.device != key.device:
+                raise RuntimeError("the caches must have the dtype and device of the nodes' keys")
+
+
+def _check_length(length, b: int, most: int, device):
+    """(device length or None, int length): the cached tokens of every sequence."""
+    if isinstance(length, torch.Tensor):
+        if length.dtype != torch.int32 or length.ndim > 1 or length.numel() not in (1, b) or length.device != device:
+            raise ValueError("a tensor length must be int32 of one element or one per sequence, on the nodes' device")
+        return length, 0
+    if not 0 <= length <= most:
+        raise ValueError(f"length {length} outside [0, {most}]")
+    return None, int(length)
+
+
+def _check_tree(parents, length, b: int, n: int, most: int, device):
+    if parents.dtype != torch.int32 or tuple(parents.shape) not in ((n,), (b, n)):
+        raise ValueError(f"parents must be int32 of shape [{n}] or [{b}, {n}] (got {parents.dtype}, {list(parents.shape)})")
+    if parents.device != device:
+        raise RuntimeError("parents must be on the device of query")
+    return _check_length(length, b, most, device)
+
+
+# ---------------------------------------------------------------------------
 # validation (triton_attention.py:14-23) and argument preparation
 # ---------------------------------------------------------------------------
 def _validate(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, repeats: int) -> None:
@@ -462,6 +619,30 @@ def _gqa_attn_decode_fake(q, k_cache, v_cache, length, scale):
     return q.new_empty(q.shape)
 
 
+# length_dev [1] or [B] int32, or None with an int length; parents [N] or [B, N] int32
+_LIB.define("tree_rope(Tensor q, Tensor k, Tensor cos, Tensor sin, Tensor? length_dev, SymInt length, Tensor parents) "
+            "-> (Tensor, Tensor)")
+_LIB.define("tree_attn(Tensor q, Tensor k, Tensor v, Tensor k_cache, Tensor v_cache, Tensor? length_dev, SymInt length, "
+            "Tensor parents, float scale) -> Tensor")
+_LIB.define("tree_commit(Tensor[] keys, Tensor[] values, Tensor path, Tensor count, Tensor? length_dev, SymInt length, "
+            "Tensor(a!)[] key_caches, Tensor(b!)[] value_caches) -> ()")
+
+
+@torch.library.register_fake("mega_trading_amd::tree_rope")
+def _tree_rope_fake(q, k, cos, sin, length_dev, length, parents):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.register_fake("mega_trading_amd::tree_attn")
+def _tree_attn_fake(q, k, v, k_cache, v_cache, length_dev, length, parents, scale):
+    return q.new_empty(q.shape)
+
+
+@torch.library.register_fake("mega_trading_amd::tree_commit")
+def _tree_commit_fake(keys, values, path, count, length_dev, length, key_caches, value_caches):
+    return None
+
+
 # the ops as the functions above call them
 _OPS = torch.ops.mega_trading_amd
 _attn_fwd = _OPS.gqa_attn_fwd.default
@@ -471,3 +652,6 @@ _attn_decode = _OPS.gqa_attn_decode.default
 _attn_decode_dev = _OPS.gqa_attn_decode_dev.default
 _rope_append = _OPS.decode_rope_append.default
 _attn_decode_append = _OPS.gqa_attn_decode_append.default
+_tree_rope = _OPS.tree_rope.default
+_tree_attn = _OPS.tree_attn.default
+_tree_commit = _OPS.tree_commit.default

@@ -1,0 +1,251 @@
+// Distillation from a teacher's top logits, forward and backward, for gfx950.
+//
+// Row r has K entries (index i_j, teacher logit y_j); an index below 0 or a logit of
+// -inf is no entry, and a row without entries counts nothing.  With the temperature T,
+//   p = softmax(y / T) over the entries,  log q = log softmax(x / T) over the vocabulary,
+//   loss = T^2 / n sum_r sum_j p_j (log p_j - log q[i_j]),  n = rows with entries,
+//   dx = g T / n (q - P),  P[v] = sum of the p_j with i_j = v.
+// Entries of one index each have their own term.  An index past the vocabulary makes
+// the row NaN.
+//
+// Bound by memory: the forward reads each logit once (a running maximum and sum), the
+// backward reads it and writes its gradient once.  One workgroup of 256 threads a row,
+// 8 values a lane a step; rows need no alignment beyond their type's (an odd
+// vocabulary), since a global load of 16 bytes takes any address.
+#pragma once
+
+#include "storage.h"
+
+namespace mt {
+
+constexpr int kDistillEntries = 1024;  // of a row
+
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
+struct DistillParams {
+  const void* x;  // [rows, V], row stride ldx
+  int64_t ldx;
+  const float* teacher;  // [rows, K]
+  const int64_t* index;  // [rows, K]
+  int V, K;
+  int64_t rows;
+  float inv_t;
+  // [rows, 4]: the row's sum of p (log p - log q), the largest logit M, the sum of exp((x - M) / T)
+  // (two numbers where one, the logarithm, would lose bits with the logits' size), 1 (0 without entries)
+  float* row;
+  // backward
+  const float* count;  // n
+  const float* grad;   // incoming gradient
+  void* dx;            // [rows, V] contiguous
+};
+
+// 8 consecutive values at any element offset
+template <int DT>
+__device__ __forceinline__ void load8_any(const void* base, int64_t i, float* v) {
+  const u32x4_any* p =
+      reinterpret_cast<const u32x4_any*>(static_cast<const char*>(base) + i * (DT == ops::kDtFP32 ? 4 : 2));
+  typename ops::IO<DT>::Raw r;
+  r.w[0] = p[0];
+  if constexpr (DT == ops::kDtFP32) r.w[1] = p[1];
+  ops::IO<DT>::unpack(r, v);
+}
+template <int DT>
+__device__ __forceinline__ void store8_any(void* base, int64_t i, const float* v) {
+  u32x4_any* p = reinterpret_cast<u32x4_any*>(static_cast<char*>(base) + i * (DT == ops::kDtFP32 ? 4 : 2));
+  if constexpr (DT == ops::kDtFP32) {
+    p[0] = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+    p[1] = u32x4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
+  } else {
+    using E = typename std::conditional<DT == ops::kDtBF16, BF16, FP16>::type;
+    p[0] = u32x4{pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3]), pack2<E>(v[4], v[5]), pack2<E>(v[6], v[7])};
+  }
+}
+
+template <bool MAX>
+__device__ __forceinline__ float block_reduce_256(float v, float* buf) {
+  v = wave_reduce<0, MAX>(v);
+  __syncthreads();  // the previous reduction's reads are done
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return red_op<MAX>(red_op<MAX>(buf[0], buf[1]), red_op<MAX>(buf[2], buf[3]));
+}
+
+constexpr int kDistillPer = kDistillEntries / 256;  // entries of a thread
+
+struct Entries {
+  int64_t idx[kDistillPer];  // -1 where there is no entry
+  float p[kDistillPer], logp[kDistillPer];
+  bool any;
+};
+
+// The row's entries and their probabilities, entry threadIdx.x + 256 j at slot j.
+__device__ __forceinline__ Entries load_entries(const DistillParams& a, int64_t row, float* buf) {
+  Entries e;
+  float m = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < kDistillPer; ++j) {
+    const int i = threadIdx.x + 256 * j;
+    e.idx[j] = -1;
+    e.logp[j] = -INFINITY;
+    if (i < a.K) {
+      e.idx[j] = a.index[row * a.K + i];
+      if (e.idx[j] >= 0) e.logp[j] = a.teacher[row * a.K + i] * a.inv_t;
+      if (e.logp[j] == -INFINITY) e.idx[j] = -1;
+    }
+    m = fmaxf(m, e.logp[j]);
+  }
+  m = block_reduce_256<true>(m, buf);
+  // NaN logits: fmaxf passes over them, the sum does not
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < kDistillPer; ++j) {
+    e.p[j] = e.idx[j] < 0 ? 0.f : expf(e.logp[j] - m);
+    sum += e.p[j];
+  }
+  sum = block_reduce_256<false>(sum, buf);
+  e.any = !(sum == 0.f);
+  const float inv = 1.f / sum, off = m + logf(sum);
+#pragma unroll
+  for (int j = 0; j < kDistillPer; ++j) {
+    e.p[j] = e.idx[j] < 0 ? 0.f : e.p[j] * inv;  // also where a NaN among the entries makes inv one
+    e.logp[j] -= off;
+  }
+  return e;
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams a) {
+  __shared__ float buf[4];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const int64_t base = row * a.ldx;
+  const Entries e = load_entries(a, row, buf);
+  if (!e.any) {
+    if (tid == 0) *reinterpret_cast<f32x4*>(a.row + 4 * row) = f32x4{0.f, 0.f, 1.f, 0.f};
+    return;
+  }
+  // a running maximum m and sum of 2^(x c - m c), c = log2(e) / T
+  const float c2 = a.inv_t * kLog2e;
+  float m = -INFINITY, s = 0.f;
+  auto add = [&](float mx, float (&v)[8]) {
+    if (mx > m) {
+      s *= exp2_fast((m - mx) * c2);
+      m = mx;
+    }
+    if (m == -INFINITY) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += exp2_fast((v[j] - m) * c2);
+  };
+  const int nvec = a.V / 8;
+  for (int c = tid; c < nvec; c += 256) {
+    float v[8];
+    load8_any<DT>(a.x, base + 8 * c, v);
+    float mx = v[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) mx = fmaxf(mx, v[j]);
+    add(mx, v);
+  }
+  if (tid < a.V - 8 * nvec) {
+    float v[8] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    v[0] = ops::IO<DT>::load1(a.x, base + 8 * nvec + tid);
+    add(v[0], v);
+  }
+  const float M = block_reduce_256<true>(m, buf);
+  s = block_reduce_256<false>(m == -INFINITY ? s : s * exp2_fast((m - M) * c2), buf);
+  const float logs = logf(s);
+  float loss = 0.f;
+#pragma unroll
+  for (int j = 0; j < kDistillPer; ++j)
+    if (e.idx[j] >= 0 && e.p[j] != 0.f) {
+      const bool in = e.idx[j] < a.V;
+      const float xi = ops::IO<DT>::load1(a.x, base + (in ? e.idx[j] : 0));
+      loss += in ? e.p[j] * (e.logp[j] - ((xi - M) * a.inv_t - logs)) : __builtin_nanf("");
+    }
+  loss = block_reduce_256<false>(loss, buf);
+  if (tid == 0) *reinterpret_cast<f32x4*>(a.row + 4 * row) = f32x4{loss, M, s, 1.f};
+}
+
+// loss = T^2 sum / n and n, in a fixed order and 64 bits: one workgroup.
+__global__ __launch_bounds__(1024) void distill_sum_kernel(const float* row, int64_t rows, float t2, float* loss,
+                                                           float* count) {
+  __shared__ double part[2][16];
+  double s = 0., n = 0.;
+  for (int64_t i = threadIdx.x; i < rows; i += 1024) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(row + 4 * i);
+    s += v[0];
+    n += v[3];
+  }
+  for (int o = 32; o > 0; o >>= 1) {
+    s += __shfl_xor(s, o, 64);
+    n += __shfl_xor(n, o, 64);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    part[0][threadIdx.x >> 6] = s;
+    part[1][threadIdx.x >> 6] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = n = 0.;
+    for (int w = 0; w < 16; ++w) {
+      s += part[0][w];
+      n += part[1][w];
+    }
+    *loss = n > 0. ? (float)(s * t2 / n) : 0.f;
+    *count = (float)n;
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
+  __shared__ float buf[4];
+  __shared__ int64_t idx[kDistillEntries];
+  __shared__ float prob[kDistillEntries];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const int64_t base = row * a.ldx, out = row * a.V;
+  const int nvec = a.V / 8;
+  const f32x4 r = *reinterpret_cast<const f32x4*>(a.row + 4 * row);
+  if (r[3] == 0.f) {
+    const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int c = tid; c < nvec; c += 256) store8_any<DT>(a.dx, out + 8 * c, z);
+    if (tid < a.V - 8 * nvec) ops::IO<DT>::store1(a.dx, out + 8 * nvec + tid, 0.f);
+    return;
+  }
+  const Entries e = load_entries(a, row, buf);
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < kDistillPer; ++j) {
+    const int i = tid + 256 * j;
+    idx[i] = e.idx[j];
+    prob[i] = e.p[j];
+    bad |= e.p[j] != 0.f && e.idx[j] >= a.V;
+  }
+  const float c2 = a.inv_t * kLog2e, M = r[1], inv = 1.f / r[2];
+  float scale = *a.grad / (*a.count * a.inv_t);
+  if (__syncthreads_or(bad)) scale = __builtin_nanf("");
+  const float qs = inv * scale;
+  for (int c = tid; c < nvec; c += 256) {
+    float v[8];
+    load8_any<DT>(a.x, base + 8 * c, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = exp2_fast((v[j] - M) * c2) * qs;
+    store8_any<DT>(a.dx, out + 8 * c, v);
+  }
+  if (tid < a.V - 8 * nvec) {
+    const int i = 8 * nvec + tid;
+    ops::IO<DT>::store1(a.dx, out + i, exp2_fast((ops::IO<DT>::load1(a.x, base + i) - M) * c2) * qs);
+  }
+  // then the entries' columns, once more and whole: q minus every p of that index (entries of
+  // one index write one value); the barrier puts these stores behind the others
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kDistillPer; ++j) {
+    if (e.idx[j] < 0 || e.idx[j] >= a.V) continue;
+    float P = 0.f;
+    for (int i = 0; i < a.K; ++i) P += idx[i] == e.idx[j] ? prob[i] : 0.f;
+    const float q = exp2_fast((ops::IO<DT>::load1(a.x, base + e.idx[j]) - M) * c2) * inv;
+    ops::IO<DT>::store1(a.dx, out + e.idx[j], (q - P) * scale);
+  }
+}
+
+}  // namespace mt

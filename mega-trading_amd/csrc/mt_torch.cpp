@@ -281,12 +281,188 @@ at::Tensor gqa_attn_decode_append(const at::Tensor& q, const at::Tensor& k, cons
   return out;
 }
 
-// --- row operators (schemas in ops.py, projection.py) ------------------------
+// contiguous and 16-byte aligned
 at::Tensor flat(const at::Tensor& x) {
   const at::Tensor c = x.contiguous();
   return aligned16(c) ? c : c.clone();
 }
 
+// --- a tree of drafted tokens (schemas in attention.py, ops.py) ---------------
+// parents [N] or [B, N] and length_dev [1] or [B] as the C ABI takes them
+struct Tree {
+  at::Tensor parents, length;
+  int64_t parents_stride;
+  int length_stride;
+  const int* length_dev() const { return length.defined() ? static_cast<const int*>(length.data_ptr()) : nullptr; }
+  const int* parent() const { return static_cast<const int*>(parents.data_ptr()); }
+};
+Tree tree(const std::optional<at::Tensor>& parents, const std::optional<at::Tensor>& length_dev) {
+  Tree t{};
+  if (parents.has_value()) {
+    t.parents = parents->contiguous();
+    t.parents_stride = t.parents.dim() == 2 ? t.parents.size(1) : 0;
+  }
+  if (length_dev.has_value() && length_dev->defined()) {
+    t.length = length_dev->contiguous();
+    t.length_stride = t.length.numel() > 1 ? 1 : 0;
+  }
+  return t;
+}
+
+// in place where the kernels can read it, else a copy
+at::Tensor rows16(const at::Tensor& t) { return kernel_ready(t) ? t : flat(t); }
+
+std::tuple<at::Tensor, at::Tensor> tree_rope(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& cos,
+                                             const at::Tensor& sin, const std::optional<at::Tensor>& length_dev,
+                                             int64_t length, const at::Tensor& parents) {
+  const c10::DeviceGuard guard(q_in.device());
+  const at::Tensor q = rows16(q_in), k = rows16(k_in);
+  const int64_t b = q.size(0), hq = q.size(1), n = q.size(2), d = q.size(3), hkv = k.size(1);
+  const at::Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+  const at::Tensor cs = flat(cos.to(at::kFloat)), sn = flat(sin.to(at::kFloat));
+  const Tree t = tree(parents, length_dev);
+  std::array<int64_t, 8> s{};
+  put_strides(s.data(), q);
+  put_strides(s.data() + 4, k);
+  s[3] = s[7] = 1;
+  check_rc(mt_tree_rope(q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), s.data(), f32_ptr(cs), f32_ptr(sn),
+                        int(std::min(cs.numel(), sn.numel()) / (d / 2)), t.parent(), t.parents_stride, t.length_dev(),
+                        t.length_stride, int(length), int(b), int(hq), int(hkv), int(n), int(d), dtype_code(q),
+                        stream_of(q)),
+           "mt_tree_rope");
+  return {qo, ko};
+}
+
+at::Tensor tree_attn(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& kc_in,
+                     const at::Tensor& vc_in, const std::optional<at::Tensor>& length_dev, int64_t length,
+                     const at::Tensor& parents, double scale) {
+  const c10::DeviceGuard guard(q_in.device());
+  const at::Tensor q = rows16(q_in), k = rows16(k_in), v = rows16(v_in), kc = rows16(kc_in), vc = rows16(vc_in);
+  const int64_t b = q.size(0), hq = q.size(1), n = q.size(2), d = q.size(3), hkv = k.size(1), cap = kc.size(2);
+  const at::Tensor out = at::empty(q.sizes(), q.options());
+  const Tree t = tree(parents, length_dev);
+  const size_t need = mt_tree_attn_workspace_size(int(b), int(hq), int(hkv), int(n), int(t.length.defined() ? cap : length),
+                                                  int(d));
+  const at::Tensor ws = at::empty({int64_t(need)}, q.options().dtype(at::kByte));
+  std::array<int64_t, 20> s{};
+  const at::Tensor* ts[5] = {&q, &k, &v, &kc, &vc};
+  for (int i = 0; i < 5; ++i) {
+    put_strides(s.data() + 4 * i, *ts[i]);
+    s[4 * i + 3] = 1;
+  }
+  check_rc(mt_tree_attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr(), out.data_ptr(), s.data(),
+                        t.parent(), t.parents_stride, t.length_dev(), t.length_stride, int(length), int(cap), int(b),
+                        int(hq), int(hkv), int(n), int(d), float(scale), dtype_code(q), need ? ws.data_ptr() : nullptr,
+                        need, stream_of(q)),
+           "mt_tree_attn");
+  return out;
+}
+
+void tree_commit(at::TensorList keys, at::TensorList values, const at::Tensor& path_in, const at::Tensor& count_in,
+                 const std::optional<at::Tensor>& length_dev, int64_t length, at::TensorList key_caches,
+                 at::TensorList value_caches) {
+  TORCH_CHECK(!keys.empty() && keys.size() == values.size() && keys.size() == key_caches.size() &&
+                  keys.size() == value_caches.size(),
+              "keys, values and the caches must hold one tensor per layer");
+  const c10::DeviceGuard guard(keys[0].device());
+  const at::Tensor path = path_in.contiguous(), count = count_in.contiguous();
+  const Tree t = tree(std::nullopt, length_dev);
+  const int64_t b = keys[0].size(0), hkv = keys[0].size(1), n = keys[0].size(2), d = keys[0].size(3);
+  auto unit = [](const at::Tensor& x) { return x.stride(3) == 1 ? x : x.contiguous(); };
+  std::vector<at::Tensor> held;  // nodes made contiguous
+  std::vector<const void*> src[2];
+  std::vector<void*> dst[2];
+  std::array<int64_t, 16> s{}, s0{};
+  auto flush = [&]() {
+    if (src[0].empty()) return;
+    check_rc(mt_tree_commit(src[0].data(), src[1].data(), dst[0].data(), dst[1].data(), int(src[0].size()), s0.data(),
+                            static_cast<const int*>(path.data_ptr()), static_cast<const int*>(count.data_ptr()),
+                            t.length_dev(), t.length_stride, int(length), int(key_caches[0].size(2)), int(b), int(hkv),
+                            int(n), int(d), dtype_code(keys[0]), stream_of(keys[0])),
+             "mt_tree_commit");
+    for (int i = 0; i < 2; ++i) {
+      src[i].clear();
+      dst[i].clear();
+    }
+  };
+  for (size_t l = 0; l < keys.size(); ++l) {
+    held.push_back(unit(keys[l]));
+    held.push_back(unit(values[l]));
+    const at::Tensor ts[4] = {held[2 * l], held[2 * l + 1], key_caches[l], value_caches[l]};
+    for (int i = 0; i < 4; ++i) {
+      put_strides(s.data() + 4 * i, ts[i]);
+      s[4 * i + 3] = 1;
+    }
+    if (s != s0) flush();  // layers of one layout share a launch
+    s0 = s;
+    for (int i = 0; i < 2; ++i) {
+      src[i].push_back(ts[i].data_ptr());
+      dst[i].push_back(ts[2 + i].data_ptr());
+    }
+  }
+  flush();
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> topk_verify(const at::Tensor& logits, const std::optional<at::Tensor>& draft,
+                                                           const at::Tensor& tokens_in, const at::Tensor& parents,
+                                                           const at::Tensor& uniform_in, const at::Tensor& noise,
+                                                           int64_t k) {
+  const c10::DeviceGuard guard(logits.device());
+  auto unit = [](const at::Tensor& x) { return x.stride(-1) == 1 ? x : x.contiguous(); };
+  const bool drafted = draft.has_value() && draft->defined();
+  const at::Tensor x = unit(logits), y = drafted ? unit(*draft) : x, e = unit(noise);
+  const at::Tensor tokens = tokens_in.contiguous(), uniform = uniform_in.contiguous();
+  const int64_t b = x.size(0), n = x.size(1), v = x.size(2);
+  const at::Tensor path = at::empty({b, n}, tokens.options().dtype(at::kInt)), count = at::empty({b}, path.options());
+  const at::Tensor token = at::empty({b, 1}, tokens.options());
+  const size_t need = mt_topk_verify_workspace_size(int(b), int(n), int(v), int(k), drafted ? 1 : 0);
+  const at::Tensor ws = at::empty({int64_t(need)}, x.options().dtype(at::kByte));
+  const Tree t = tree(parents, std::nullopt);
+  const int64_t s[4] = {x.stride(0), x.stride(1), y.stride(0), y.stride(1)};
+  check_rc(mt_topk_verify(x.data_ptr(), drafted ? y.data_ptr() : nullptr, s, static_cast<const int64_t*>(tokens.data_ptr()),
+                          t.parent(), t.parents_stride, f32_ptr(uniform), f32_ptr(e), e.stride(0),
+                          static_cast<int*>(path.data_ptr()), static_cast<int*>(count.data_ptr()),
+                          static_cast<int64_t*>(token.data_ptr()), int(b), int(n), int(v), int(k), dtype_code(x),
+                          ws.data_ptr(), need, stream_of(x)),
+           "mt_topk_verify");
+  return {path, count, token};
+}
+
+// --- distillation (schemas in ops.py) ----------------------------------------
+// rows of the last dim, a row stride of at least its size
+at::Tensor plain_rows(const at::Tensor& x) {
+  const at::Tensor r = x.reshape({-1, x.size(-1)});
+  return (r.stride(1) == 1 || r.size(1) == 1) && (r.size(0) < 2 || r.stride(0) >= r.size(1)) ? r : r.contiguous();
+}
+int64_t row_stride(const at::Tensor& r) { return r.size(0) > 1 ? r.stride(0) : r.size(1); }
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> topk_distill_fwd(const at::Tensor& logits, const at::Tensor& teacher,
+                                                                const at::Tensor& index, double temperature) {
+  const c10::DeviceGuard guard(logits.device());
+  const at::Tensor x = plain_rows(logits), y = teacher.to(at::kFloat).contiguous(), i = index.to(at::kLong).contiguous();
+  const auto f32 = x.options().dtype(at::kFloat);
+  const at::Tensor loss = at::empty({}, f32), state = at::empty({x.size(0), 4}, f32), count = at::empty({}, f32);
+  check_rc(mt_topk_distill_fwd(x.data_ptr(), row_stride(x), f32_ptr(y), static_cast<const int64_t*>(i.data_ptr()),
+                               x.size(0), int(x.size(1)), int(y.size(-1)), float(temperature), f32_ptr(state),
+                               f32_ptr(loss), f32_ptr(count), dtype_code(x), stream_of(x)),
+           "mt_topk_distill_fwd");
+  return {loss, state, count};
+}
+
+at::Tensor topk_distill_bwd(const at::Tensor& logits, const at::Tensor& teacher, const at::Tensor& index,
+                            const at::Tensor& state, const at::Tensor& count, const at::Tensor& grad,
+                            double temperature) {
+  const c10::DeviceGuard guard(logits.device());
+  const at::Tensor x = plain_rows(logits), y = teacher.to(at::kFloat).contiguous(), i = index.to(at::kLong).contiguous();
+  const at::Tensor g = grad.to(at::kFloat).contiguous(), dx = at::empty(logits.sizes(), logits.options());
+  check_rc(mt_topk_distill_bwd(x.data_ptr(), row_stride(x), f32_ptr(y), static_cast<const int64_t*>(i.data_ptr()),
+                               f32_ptr(state), f32_ptr(count), f32_ptr(g), dx.data_ptr(), x.size(0), int(x.size(1)),
+                               int(y.size(-1)), float(temperature), dtype_code(x), stream_of(x)),
+           "mt_topk_distill_bwd");
+  return dx;
+}
+
+// --- row operators (schemas in ops.py, projection.py) ------------------------
 // x's rows of the last dim, in place where the kernels can read them
 struct Rows {
   at::Tensor t;
@@ -799,6 +975,28 @@ struct LinearCeFn : torch::autograd::Function<LinearCeFn> {
   }
 };
 
+struct DistillFn : torch::autograd::Function<DistillFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& teacher,
+                               const at::Tensor& index, double temperature) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = MT_OP(topk_distill_fwd);
+    auto [loss, state, count] = op.call(logits, teacher, index, temperature);
+    ctx->save_for_backward({logits, teacher, index, state, count});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->mark_non_differentiable({state, count});
+    ctx->set_materialize_grads(false);
+    return {loss, state, count};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    if (!g[0].defined() || !ctx->needs_input_grad(0)) return variable_list(4);
+    const auto s = ctx->get_saved_variables();
+    static const auto op = MT_OP(topk_distill_bwd);
+    variable_list r(4);
+    r[0] = op.call(s[0], s[1], s[2], s[3], s[4], g[0], ctx->saved_data["temperature"].toDouble());
+    return r;
+  }
+};
+
 // Whether a call records a gradient: without one the op runs below autograd
 // directly.  RoPE tables that require one record the call too (and get none).
 template <class... T>
@@ -886,6 +1084,26 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> fused_linear_ce_ad(const at::Tens
   return {r[0], r[1], r[2]};
 }
 
+std::tuple<at::Tensor, at::Tensor, at::Tensor> topk_distill_fwd_ad(const at::Tensor& logits, const at::Tensor& teacher,
+                                                                   const at::Tensor& index, double temperature) {
+  if (!records(logits, teacher)) MT_BELOW(topk_distill_fwd, logits, teacher, index, temperature);
+  auto r = DistillFn::apply(logits, teacher, index, temperature);
+  return {r[0], r[1], r[2]};
+}
+
+// The write into the caches has no result that could carry a refusal: it refuses at once.
+void tree_commit_ad(at::TensorList keys, at::TensorList values, const at::Tensor& path, const at::Tensor& count,
+                    const std::optional<at::Tensor>& length_dev, int64_t length, at::TensorList key_caches,
+                    at::TensorList value_caches) {
+  if (c10::GradMode::is_enabled())
+    for (const at::TensorList& l : {keys, values, key_caches, value_caches})
+      for (const at::Tensor& t : l)
+        TORCH_CHECK(!t.requires_grad(), "mega_trading_amd::tree_commit has no autograd formula: call it under no_grad");
+  at::AutoDispatchBelowAutograd below;
+  static const auto op = MT_OP(tree_commit);
+  op.call(keys, values, path, count, length_dev, length, key_caches, value_caches);
+}
+
 // An op without a formula (the backward ops among them: no double backward)
 // refuses a gradient instead of dropping it: its outputs' node raises.  torch's
 // own fallback for such ops only warns and passes no gradient on.  Caches that an
@@ -932,7 +1150,10 @@ void count_writes(const c10::OperatorHandle& op, c10::DispatchKeySet ks, torch::
   variable_list written;
   for (size_t i = 0; i < params.size(); ++i) {
     const c10::IValue& a = torch::jit::peek(*stack, i, params.size());
-    if (params[i].alias_info() && params[i].alias_info()->isWrite() && a.isTensor()) written.push_back(a.toTensor());
+    if (!params[i].alias_info() || !params[i].alias_info()->isWrite()) continue;
+    if (a.isTensor()) written.push_back(a.toTensor());
+    else if (a.isTensorList())
+      for (const at::Tensor& t : a.toTensorList()) written.push_back(t);
   }
   {
     at::AutoDispatchBelowADInplaceOrView below;
@@ -948,9 +1169,12 @@ TORCH_LIBRARY_IMPL(mega_trading_amd, Autograd, m) {
   // gqa_attn_bwd_packed keeps torch's fallback, a warning, which it has always had
   for (const char* op : {"gqa_attn_bwd", "gqa_attn_decode", "gqa_attn_decode_dev", "decode_rope_append",
                          "gqa_attn_decode_append", "rms_norm_bwd", "add_rms_norm_bwd", "rms_norm_bwd_mixed", "swiglu_bwd",
-                         "swiglu_packed_bwd", "topk_sample", "linear_rows", "linear_rows_gate", "ce_sum", "scale_pair"})
+                         "swiglu_packed_bwd", "topk_sample", "linear_rows", "linear_rows_gate", "ce_sum", "scale_pair",
+                         "tree_rope", "tree_attn", "topk_verify", "topk_distill_bwd"})
     m.impl(op, torch::CppFunction::makeFromBoxedFunction<&no_formula>());
   m.impl("fused_linear_ce", &fused_linear_ce_ad);
+  m.impl("topk_distill_fwd", &topk_distill_fwd_ad);
+  m.impl("tree_commit", &tree_commit_ad);
   m.impl("gqa_attn_fwd", &gqa_attn_fwd_ad);
   m.impl("gqa_rope_attn_fwd", &gqa_rope_attn_fwd_ad);
   m.impl("gqa_rope_attn_packed_fwd", &gqa_rope_attn_packed_fwd_ad);
@@ -964,7 +1188,7 @@ TORCH_LIBRARY_IMPL(mega_trading_amd, Autograd, m) {
 }
 
 TORCH_LIBRARY_IMPL(mega_trading_amd, ADInplaceOrView, m) {
-  for (const char* op : {"decode_rope_append", "gqa_attn_decode_append"})
+  for (const char* op : {"decode_rope_append", "gqa_attn_decode_append", "tree_commit"})
     m.impl(op, torch::CppFunction::makeFromBoxedFunction<&count_writes>());
 }
 
@@ -991,6 +1215,12 @@ TORCH_LIBRARY_IMPL(mega_trading_amd, CUDA, m) {
   m.impl("swiglu_packed_bwd", &swiglu_packed_bwd);
   m.impl("rope_fwd", &rope_fwd);
   m.impl("topk_sample", &topk_sample);
+  m.impl("tree_rope", &tree_rope);
+  m.impl("tree_attn", &tree_attn);
+  m.impl("tree_commit", &tree_commit);
+  m.impl("topk_verify", &topk_verify);
+  m.impl("topk_distill_fwd", &topk_distill_fwd);
+  m.impl("topk_distill_bwd", &topk_distill_bwd);
   m.impl("linear_rows", &linear_rows);
   m.impl("linear_rows_gate", &linear_rows_gate);
   m.impl("ce_count", &ce_count);

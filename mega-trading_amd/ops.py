@@ -27,13 +27,16 @@ from __future__ import annotations
 import torch
 
 from . import _native
+from .attention import MAX_TREE_NODES
 from .gemm_tuning import tuned_gemms
 
 __all__ = ["rms_norm", "add_rms_norm", "rms_norm_mixed", "add_rms_norm_mixed", "swiglu_gate", "swiglu_gate_packed",
-           "apply_rope", "fused_linear_cross_entropy", "topk_sample", "MAX_NORM_DIM", "MAX_SAMPLE_VOCAB"]
+           "apply_rope", "fused_linear_cross_entropy", "topk_sample", "topk_verify", "topk_distillation", "MAX_NORM_DIM",
+           "MAX_SAMPLE_VOCAB", "MAX_TEACHER_ENTRIES"]
 
 MAX_NORM_DIM = 4096
 MAX_SAMPLE_VOCAB = 32768  # vocabulary of one topk_sample row (1024 threads x 32 values in registers)
+MAX_TEACHER_ENTRIES = 1024  # teacher logits of one topk_distillation row
 _DT = {torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_FP16, torch.float32: _native.DTYPE_FP32}
 _DTYPE_OF = {v: k for k, v in _DT.items()}
 
@@ -248,6 +251,97 @@ def topk_sample(logits: torch.Tensor, noise: torch.Tensor, k: int) -> torch.Tens
     return _topk_sample(logits, noise, k)
 
 
+def topk_verify(
+    logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, uniform: torch.Tensor, noise: torch.Tensor, k: int, *,
+    draft_logits: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Verify a tree of drafted tokens against the target's top-k distribution and
+    draw the token after it: ``(path, count, token)``.
+
+    Row n of ``logits`` [B, N, vocab] (bf16, fp16 or fp32) holds the target's logits
+    after node n, ``tokens`` [B, N] int64 the nodes' tokens, ``parents`` int32 [N]
+    or [B, N] their parents (an earlier node; -1 for node 0, the token already
+    accepted last, where the walk starts; anything else is padding, which is not
+    visited).  At node u, p is the softmax over the logits >= the k-th largest of
+    row u (ties included, as ``topk_sample``) and q the same of row u of
+    ``draft_logits``, the logits that u's children were drawn from with the same k.
+    The children are tried in index order: child c with token x is accepted if
+    ``uniform[b, c] * q[x] < p[x]`` and the walk goes on from it; else p becomes
+    ``max(p - q, 0)``, scaled to sum 1.  Without ``draft_logits`` q is 1 at x:
+    children that were picked, not drawn.  After the last child the token is the
+    first index of the largest ``p / noise``.
+
+    With ``uniform`` [B, N] fp32 from [0, 1) (``torch.rand``) and ``noise``
+    [B, vocab] fp32 Exponential(1) draws, the accepted tokens and the drawn one are
+    distributed as the target's own draws; for one node this is ``topk_sample``.
+
+    ``path`` [B, N] int32 holds the accepted nodes in order (node 0 first, -1 behind
+    them), ``count`` [B] int32 their number, ``token`` [B, 1] int64 the drawn token.
+    A sequence whose node 0 is padding has count 0 and token 0.  NaN and -inf logits
+    count as the lowest fp32 value, +inf as the highest."""
+    _check_device_dtype(logits, "logits")
+    if logits.ndim != 3:
+        raise ValueError("logits must have shape [batch, nodes, vocab]")
+    b, n, vocab = logits.shape
+    if not 1 <= n <= MAX_TREE_NODES:
+        raise ValueError(f"need 1 to {MAX_TREE_NODES} nodes (got {n})")
+    if not 1 <= k <= vocab or vocab > MAX_SAMPLE_VOCAB:
+        raise ValueError(f"need 1 <= k <= vocab <= {MAX_SAMPLE_VOCAB} (k={k}, vocab={vocab})")
+    for name, t, dtype, shapes in (("tokens", tokens, torch.int64, ((b, n),)), ("parents", parents, torch.int32, ((n,), (b, n))),
+                                   ("uniform", uniform, torch.float32, ((b, n),)),
+                                   ("noise", noise, torch.float32, ((b, vocab),))):
+        if t.dtype != dtype or tuple(t.shape) not in shapes:
+            raise ValueError(f"{name} must be {dtype} of shape {list(shapes[-1])} (got {t.dtype}, {list(t.shape)})")
+        if t.device != logits.device:
+            raise RuntimeError(f"{name} must be on the device of logits")
+    if draft_logits is not None:
+        if draft_logits.shape != logits.shape:
+            raise ValueError("draft_logits must have the shape of logits")
+        if draft_logits.dtype != logits.dtype or draft_logits.device != logits.device:
+            raise RuntimeError("draft_logits must have the dtype and device of logits")
+    _native.ensure()
+    return _topk_verify(logits, draft_logits, tokens, parents, uniform, noise, k)
+
+
+def topk_distillation(
+    logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_indices: torch.Tensor, *, temperature: float = 1.0
+) -> torch.Tensor:
+    """Mean distillation loss of student ``logits`` [..., vocab] against a
+    teacher's top logits: ``teacher_logits`` [..., K] (K <= 1024) at the vocabulary
+    ``teacher_indices`` [..., K] (int32/int64).
+
+    Per row, with T = ``temperature`` and p = softmax(teacher_logits / T) over the
+    row's entries, the loss is T^2 sum_j p_j (log p_j - log softmax(logits / T)[index_j]):
+    the divergence from the student's distribution over the whole vocabulary to the
+    teacher's over its entries.  An index below 0 (or a teacher logit of -inf) is no
+    entry; rows without entries contribute nothing (none left: loss 0, zero
+    gradients).  Entries that share an index each have their own term.  An index
+    past the vocabulary makes its row NaN.
+
+    ``logits`` and ``teacher_logits`` are bf16, fp16 or fp32, any vocabulary size;
+    arithmetic and the scalar loss are fp32.  The gradient is the student's alone,
+    rounded once to its dtype; the teacher gets none."""
+    _check_device_dtype(logits, "logits")
+    _check_device_dtype(teacher_logits, "teacher_logits")
+    if logits.ndim < 1 or logits.shape[-1] < 1:
+        raise ValueError("logits must have shape [..., vocab]")
+    if teacher_logits.shape[:-1] != logits.shape[:-1] or teacher_logits.ndim != logits.ndim:
+        raise ValueError("teacher_logits must have shape [..., entries] with the rows of logits")
+    if teacher_indices.shape != teacher_logits.shape:
+        raise ValueError("teacher_indices must have the shape of teacher_logits")
+    if teacher_indices.dtype not in (torch.int32, torch.int64):
+        raise ValueError("teacher_indices must be an integer tensor (int32 or int64)")
+    if not 1 <= teacher_logits.shape[-1] <= MAX_TEACHER_ENTRIES:
+        raise ValueError(f"need 1 to {MAX_TEACHER_ENTRIES} teacher logits a row (got {teacher_logits.shape[-1]})")
+    if teacher_logits.device != logits.device or teacher_indices.device != logits.device:
+        raise RuntimeError("the teacher's tensors must be on the device of logits")
+    if not 1e-30 < temperature < 1e30:
+        raise ValueError(f"temperature must be positive and finite (got {temperature})")
+    _native.ensure()
+    loss, _state, _count = _topk_distill_fwd(logits, teacher_logits, teacher_indices, float(temperature))
+    return loss
+
+
 # ---------------------------------------------------------------------------
 # the ops: schemas and shapes here, GPU kernels and autograd in libmt_torch.so
 # ---------------------------------------------------------------------------
@@ -272,6 +366,12 @@ _LIB.define("swiglu_packed_bwd(Tensor gate_up, Tensor dout) -> Tensor")
 # query and key in one launch, outputs in the inputs' layout; inverse rotates by -theta (the backward)
 _LIB.define("rope_fwd(Tensor query, Tensor key, Tensor cos, Tensor sin, bool inverse) -> (Tensor, Tensor)")
 _LIB.define("topk_sample(Tensor logits, Tensor noise, SymInt k) -> Tensor")
+_LIB.define("topk_verify(Tensor logits, Tensor? draft_logits, Tensor tokens, Tensor parents, Tensor uniform, Tensor noise, "
+            "SymInt k) -> (Tensor, Tensor, Tensor)")
+# (loss fp32 scalar, row state fp32 [rows, 4], rows with entries fp32 scalar); the last two feed the backward
+_LIB.define("topk_distill_fwd(Tensor logits, Tensor teacher, Tensor index, float temperature) -> (Tensor, Tensor, Tensor)")
+_LIB.define("topk_distill_bwd(Tensor logits, Tensor teacher, Tensor index, Tensor row_state, Tensor count, Tensor grad, "
+            "float temperature) -> Tensor")
 
 
 def _like(x, dtype=None):
@@ -346,6 +446,25 @@ def _rope_fwd_fake(query, key, cos, sin, inverse):
 @torch.library.register_fake("mega_trading_amd::topk_sample")
 def _topk_sample_fake(logits, noise, k):
     return logits.new_empty((logits.shape[0], 1), dtype=torch.int64)
+
+
+@torch.library.register_fake("mega_trading_amd::topk_verify")
+def _topk_verify_fake(logits, draft_logits, tokens, parents, uniform, noise, k):
+    b, n = tokens.shape
+    return (tokens.new_empty((b, n), dtype=torch.int32), tokens.new_empty((b,), dtype=torch.int32),
+            tokens.new_empty((b, 1)))
+
+
+@torch.library.register_fake("mega_trading_amd::topk_distill_fwd")
+def _topk_distill_fwd_fake(logits, teacher, index, temperature):
+    f32 = dict(dtype=torch.float32)
+    return (logits.new_empty((), **f32), logits.new_empty((logits.numel() // logits.shape[-1], 4), **f32),
+            logits.new_empty((), **f32))
+
+
+@torch.library.register_fake("mega_trading_amd::topk_distill_bwd")
+def _topk_distill_bwd_fake(logits, teacher, index, row_state, count, grad, temperature):
+    return _like(logits)
 
 
 # Logits bytes per chunk.  Measured at the C5 shape (32768 x 16384 bf16 logits,
@@ -436,6 +555,8 @@ _swiglu_fwd = _OPS.swiglu_fwd.default
 _swiglu_packed_fwd = _OPS.swiglu_packed_fwd.default
 _rope_fwd = _OPS.rope_fwd.default
 _topk_sample = _OPS.topk_sample.default
+_topk_verify = _OPS.topk_verify.default
+_topk_distill_fwd = _OPS.topk_distill_fwd.default
 _fused_linear_ce = _OPS.fused_linear_ce.default
 _ce_count = _OPS.ce_count.default
 _ce_sum = _OPS.ce_sum.default
