@@ -19,8 +19,7 @@
 namespace mt {
 
 constexpr int kDistillEntries = 1024;  // of a row
-
-typedef u32x4 u32x4_any __attribute__((aligned(2)));
+constexpr int kDistillAhead = 4;       // loads of a thread in flight
 
 struct DistillParams {
   const void* x;  // [rows, V], row stride ldx
@@ -38,28 +37,6 @@ struct DistillParams {
   const float* grad;   // incoming gradient
   void* dx;            // [rows, V] contiguous
 };
-
-// 8 consecutive values at any element offset
-template <int DT>
-__device__ __forceinline__ void load8_any(const void* base, int64_t i, float* v) {
-  const u32x4_any* p =
-      reinterpret_cast<const u32x4_any*>(static_cast<const char*>(base) + i * (DT == ops::kDtFP32 ? 4 : 2));
-  typename ops::IO<DT>::Raw r;
-  r.w[0] = p[0];
-  if constexpr (DT == ops::kDtFP32) r.w[1] = p[1];
-  ops::IO<DT>::unpack(r, v);
-}
-template <int DT>
-__device__ __forceinline__ void store8_any(void* base, int64_t i, const float* v) {
-  u32x4_any* p = reinterpret_cast<u32x4_any*>(static_cast<char*>(base) + i * (DT == ops::kDtFP32 ? 4 : 2));
-  if constexpr (DT == ops::kDtFP32) {
-    p[0] = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-    p[1] = u32x4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
-  } else {
-    using E = typename std::conditional<DT == ops::kDtBF16, BF16, FP16>::type;
-    p[0] = u32x4{pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3]), pack2<E>(v[4], v[5]), pack2<E>(v[6], v[7])};
-  }
-}
 
 template <bool MAX>
 __device__ __forceinline__ float block_reduce_256(float v, float* buf) {
@@ -137,13 +114,20 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams a) {
     for (int j = 0; j < 8; ++j) s += exp2_fast((v[j] - m) * c2);
   };
   const int nvec = a.V / 8;
-  for (int c = tid; c < nvec; c += 256) {
-    float v[8];
-    load8_any<DT>(a.x, base + 8 * c, v);
-    float mx = v[0];
+  for (int c0 = tid; c0 < nvec; c0 += 256 * kDistillAhead) {
+    typename ops::IO<DT>::Raw r[kDistillAhead];
 #pragma unroll
-    for (int j = 1; j < 8; ++j) mx = fmaxf(mx, v[j]);
-    add(mx, v);
+    for (int i = 0; i < kDistillAhead; ++i) r[i] = ops::load8_any<DT>(a.x, base + 8 * min(c0 + 256 * i, nvec - 1));
+#pragma unroll
+    for (int i = 0; i < kDistillAhead; ++i) {
+      if (c0 + 256 * i >= nvec) continue;
+      float v[8];
+      ops::IO<DT>::unpack(r[i], v);
+      float mx = v[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) mx = fmaxf(mx, v[j]);
+      add(mx, v);
+    }
   }
   if (tid < a.V - 8 * nvec) {
     float v[8] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -170,10 +154,16 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* row, int
                                                            float* count) {
   __shared__ double part[2][16];
   double s = 0., n = 0.;
-  for (int64_t i = threadIdx.x; i < rows; i += 1024) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(row + 4 * i);
-    s += v[0];
-    n += v[3];
+  for (int64_t i = threadIdx.x; i < rows; i += 8 * 1024) {
+    f32x4 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const f32x4*>(row + 4 * min(i + 1024 * j, rows - 1));
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i + 1024 * j < rows) {
+        s += v[j][0];
+        n += v[j][3];
+      }
   }
   for (int o = 32; o > 0; o >>= 1) {
     s += __shfl_xor(s, o, 64);
@@ -207,7 +197,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
   const f32x4 r = *reinterpret_cast<const f32x4*>(a.row + 4 * row);
   if (r[3] == 0.f) {
     const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int c = tid; c < nvec; c += 256) store8_any<DT>(a.dx, out + 8 * c, z);
+    for (int c = tid; c < nvec; c += 256) ops::store8_any<DT>(a.dx, out + 8 * c, z);
     if (tid < a.V - 8 * nvec) ops::IO<DT>::store1(a.dx, out + 8 * nvec + tid, 0.f);
     return;
   }
@@ -224,12 +214,19 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
   float scale = *a.grad / (*a.count * a.inv_t);
   if (__syncthreads_or(bad)) scale = __builtin_nanf("");
   const float qs = inv * scale;
-  for (int c = tid; c < nvec; c += 256) {
-    float v[8];
-    load8_any<DT>(a.x, base + 8 * c, v);
+  for (int c0 = tid; c0 < nvec; c0 += 256 * kDistillAhead) {
+    typename ops::IO<DT>::Raw r[kDistillAhead];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = exp2_fast((v[j] - M) * c2) * qs;
-    store8_any<DT>(a.dx, out + 8 * c, v);
+    for (int i = 0; i < kDistillAhead; ++i) r[i] = ops::load8_any<DT>(a.x, base + 8 * min(c0 + 256 * i, nvec - 1));
+#pragma unroll
+    for (int i = 0; i < kDistillAhead; ++i) {
+      if (c0 + 256 * i >= nvec) continue;
+      float v[8];
+      ops::IO<DT>::unpack(r[i], v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = exp2_fast((v[j] - M) * c2) * qs;
+      ops::store8_any<DT>(a.dx, out + 8 * (c0 + 256 * i), v);
+    }
   }
   if (tid < a.V - 8 * nvec) {
     const int i = 8 * nvec + tid;

@@ -107,20 +107,38 @@ void launch_tree(const mt::TreeAttnParams& p, int nt, unsigned grid, hipStream_t
   }
 }
 
-// Workspace of the verification: the rows' RowTop, then the target rows' lists.
-size_t verify_tops(int64_t B, int64_t N, bool draft) {
-  return ((size_t)(B * N) * (draft ? 2 : 1) * sizeof(mt::RowTop) + 255) / 256 * 256;
+// Nodes of a sequence whose rows are taken before the walk: as many as the card works on at a time.
+// A row of up to 16384 words leaves room for others on its CU, a longer one hardly.  Rows and walk, us:
+// 32 sequences of 16 nodes with a drafter, 16384 fp32 words, 4 rows a CU (all nodes) 21.0 + 10.5, 2 rows
+// 11.1 + 26.5, 1 row 9.0 + 32.7; 64 sequences of 64 nodes, 32001 16-bit words, 4 rows a CU 48.8 + 19.4, 2 rows
+// 25.4 + 19.3, 1 row 13.6 + 19.3.
+int verify_ahead(int64_t B, int N, int vocab, bool draft) {
+  const int64_t rows = (vocab <= 16384 ? 4 : 1) * (int64_t)device_cus();
+  return (int)std::max<int64_t>(1, std::min<int64_t>(N, rows / (B * (draft ? 2 : 1))));
 }
-bool verify_lists(int vocab, int k) { return k <= mt::kSampleWaveK && k < vocab; }
 
-template <int DT>
+// Workspace of the verification: the rows' RowTop, then the target rows' lists.
+size_t verify_tops(int64_t B, int ahead, bool draft) {
+  return ((size_t)B * ahead * (draft ? 2 : 1) * sizeof(mt::RowTop) + 255) / 256 * 256;
+}
+
+template <int DT, int T, int C>
 void launch_verify(const mt::VerifyParams& p, hipStream_t st) {
-  const dim3 rows((unsigned)((int64_t)p.B * p.N * (p.rows[1] ? 2 : 1))), block(mt::kSampleThreads);
-  if (p.V <= 8 * mt::kSampleThreads) hipLaunchKernelGGL((mt::verify_rows_kernel<DT, 8>), rows, block, 0, st, p);
-  else if (p.V <= 16 * mt::kSampleThreads) hipLaunchKernelGGL((mt::verify_rows_kernel<DT, 16>), rows, block, 0, st, p);
-  else hipLaunchKernelGGL((mt::verify_rows_kernel<DT, 32>), rows, block, 0, st, p);
-  if (p.rows[1]) hipLaunchKernelGGL((mt::verify_walk_kernel<DT, true>), dim3((unsigned)p.B), block, 0, st, p);
-  else hipLaunchKernelGGL((mt::verify_walk_kernel<DT, false>), dim3((unsigned)p.B), block, 0, st, p);
+  const dim3 rows((unsigned)((int64_t)p.B * p.ahead * (p.rows[1] ? 2 : 1))), block(T), walks((unsigned)p.B);
+  hipLaunchKernelGGL((mt::verify_rows_kernel<DT, T, C>), rows, block, 0, st, p);
+  if (p.rows[1]) hipLaunchKernelGGL((mt::verify_walk_kernel<DT, T, C, true>), walks, block, 0, st, p);
+  else hipLaunchKernelGGL((mt::verify_walk_kernel<DT, T, C, false>), walks, block, 0, st, p);
+}
+
+// A row in 32 registers a thread (at most 16 for a short vocabulary): 64 16-bit values or 32 fp32 ones.
+// More waves a row cost more than they bring (512 against 1024 threads for the rows above: 21.0 / 35.9 and
+// 49.8 / 50.7 us): what a wave does for itself, the ballots of the bound above all, is most of a row's time.
+template <int DT>
+void launch_verify_v(const mt::VerifyParams& p, hipStream_t st) {
+  constexpr bool wide = DT == kDtFP32;
+  if (p.V <= 4096) launch_verify<DT, 256, 2>(p, st);
+  else if (p.V <= 16384) launch_verify<DT, wide ? 512 : 256, wide ? 4 : 8>(p, st);
+  else launch_verify<DT, wide ? 1024 : 512, wide ? 4 : 8>(p, st);
 }
 
 int check_distill(int64_t ld, int64_t rows, int vocab, int entries, float temperature, int dtype) {
@@ -321,8 +339,8 @@ int mt_tree_commit(const void* const* keys, const void* const* values, void* con
 
 size_t mt_topk_verify_workspace_size(int B, int N, int vocab, int k, int draft) {
   if (B < 1 || N < 1 || N > mt::kTreeNodes || vocab < 1 || k < 1) return 0;
-  const size_t lists = verify_lists(vocab, k) ? (size_t)B * N * mt::kSampleCand * sizeof(mt::u32x2) : 0;
-  return verify_tops(B, N, draft != 0) + lists;
+  const int ahead = verify_ahead(B, N, vocab, draft != 0);
+  return verify_tops(B, ahead, draft != 0) + (size_t)B * ahead * mt::kVerifyList * sizeof(mt::u32x2);
 }
 
 int mt_topk_verify(const void* logits, const void* draft_logits, const int64_t* strides, const int64_t* tokens,
@@ -354,6 +372,7 @@ int mt_topk_verify(const void* logits, const void* draft_logits, const int64_t* 
   if (workspace_bytes < need)
     return fail(MT_E_WORKSPACE, "workspace of %zu bytes is smaller than the %zu required", workspace_bytes, need);
   mt::VerifyParams p{};
+  p.ahead = verify_ahead(B, N, vocab, draft_logits != nullptr);
   p.rows[0] = logits;
   p.rows[1] = draft_logits;
   for (int i = 0; i < 2; ++i) {
@@ -367,7 +386,7 @@ int mt_topk_verify(const void* logits, const void* draft_logits, const int64_t* 
   p.noise = noise;
   p.ldn = noise_row_stride;
   p.top = static_cast<mt::RowTop*>(workspace);
-  p.list = reinterpret_cast<mt::u32x2*>(static_cast<char*>(workspace) + verify_tops(B, N, draft_logits != nullptr));
+  p.list = reinterpret_cast<mt::u32x2*>(static_cast<char*>(workspace) + verify_tops(B, p.ahead, draft_logits != nullptr));
   p.path = path;
   p.count = count;
   p.token = token;
@@ -376,9 +395,9 @@ int mt_topk_verify(const void* logits, const void* draft_logits, const int64_t* 
   p.V = vocab;
   p.k = k;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == MT_DTYPE_BF16) launch_verify<kDtBF16>(p, st);
-  else if (dtype == MT_DTYPE_FP16) launch_verify<kDtFP16>(p, st);
-  else launch_verify<kDtFP32>(p, st);
+  if (dtype == MT_DTYPE_BF16) launch_verify_v<kDtBF16>(p, st);
+  else if (dtype == MT_DTYPE_FP16) launch_verify_v<kDtFP16>(p, st);
+  else launch_verify_v<kDtFP32>(p, st);
   return launched("verification");
 }
 

@@ -13,14 +13,16 @@
 // from q, or chosen without q, thus leave the target's distribution unchanged.
 // NaN and -inf logits count as the lowest float, +inf as the highest.
 //
-// Two launches.  verify_rows_kernel takes every row that the walk may need, one
-// workgroup of 1024 threads a row (held in registers as order-preserving keys,
-// EPT a thread): the k-th largest key, the maximum, the sum of the kept
-// exponentials, and, where they are few, the kept values themselves as a list.
-// verify_walk_kernel then walks, one workgroup a sequence: an acceptance needs
-// four scalars and none of the vocabulary, a rejection or the draw goes over
-// the node's list (a row without one, for k > 1024, k = vocab or many ties, is
-// read again).
+// Two launches.  verify_rows_kernel takes rows that the walk may need, one workgroup
+// a row: the k-th largest logit, the maximum, the sum of the kept exponentials, and,
+// where they are few, the kept values themselves as a list.  verify_walk_kernel then
+// walks, one workgroup a sequence: an acceptance needs four scalars and none of the
+// vocabulary, a rejection or the draw goes over the node's list (a row without one,
+// for large k or many ties, is read again).
+//
+// A walk visits a few nodes, but which is known only as it goes.  The rows of the
+// first `ahead` nodes of every sequence are taken before it, all at once: as many as
+// the card holds at a time.  A node past them is taken when the walk reaches it.
 #pragma once
 
 #include "sample_kernels.h"
@@ -45,17 +47,20 @@ struct VerifyParams {
   const float* uniform;    // [B, N]
   const float* noise;      // [B, V], row stride ldn
   int64_t ldn;
-  RowTop* top;             // workspace [2 or 1][B, N]
-  u32x2* list;             // workspace [B, N][kSampleCand]: (key, index) of the target rows
+  RowTop* top;             // workspace [2 or 1][B, ahead]
+  u32x2* list;             // workspace [B, ahead][kVerifyList]: (key, index) of the target rows
   int* path;               // [B, N]
   int* count;              // [B]
   int64_t* token;          // [B]
-  int B, N, V, k;
+  int B, N, V, k, ahead;
 };
 
+constexpr int kVerifyList = 1024;  // values of a list
+
+// A logit as the operator counts it: finite, and no negative zero (its key is another).
 template <int DT>
 __device__ __forceinline__ float load_logit(const void* base, int64_t i) {
-  return fminf(fmaxf(ops::IO<DT>::load1(base, i), -__FLT_MAX__), __FLT_MAX__);
+  return fminf(fmaxf(ops::IO<DT>::load1(base, i), -__FLT_MAX__), __FLT_MAX__) + 0.f;
 }
 
 // A node's parent, or -2 for padding: only earlier nodes have children.
@@ -64,36 +69,142 @@ __device__ __forceinline__ int verify_parent(const VerifyParams& p, int b, int n
   return up < n ? up : -2;
 }
 
+template <int T>
 struct RowLds {
-  uint32_t bound[2][kSampleWaves];
-  float top[kSampleWaves], buf[kSampleWaves];
-  int count[kSampleWaves];
+  __attribute__((aligned(16))) uint32_t key[kVerifyList];
+  int idx[kVerifyList];
+  float buf[T / 64], top[T / 64];
+  uint32_t bound[2][T / 64];
+  int count[T / 64];
   uint32_t kth;
-  __attribute__((aligned(16))) uint32_t key[kSampleCand];
-  int idx[kSampleCand];
 };
 
-// key: of value tid + 1024 j of the row at slot j, 0 past its end.  A row with a
-// list has it in s.key / s.idx on return, behind a barrier.
-template <int EPT>
-__device__ __forceinline__ RowTop row_top(const uint32_t (&key)[EPT], int V, int k, RowLds& s) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  uint32_t mx = key[0];
+// block-wide max or sum; barriers at both ends of buf's use
+template <int T, bool MAX>
+__device__ __forceinline__ float reduce_all(float v, float* buf) {
+  v = wave_reduce<0, MAX>(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float r = buf[0];
 #pragma unroll
-  for (int j = 1; j < EPT; ++j) mx = max(mx, key[j]);
-  // bounds below the k-th key: the smallest over the waves of their ceil(k / 16)-th lane
-  // maxima, the largest of their k-th ones (0 where a wave holds fewer values)
-  const bool list = k <= kSampleWaveK && k < V;
+  for (int w = 1; w < T / 64; ++w) r = red_op<MAX>(r, buf[w]);
+  return r;
+}
+
+// A row in registers as it was loaded: slot 8 c + e of a thread holds value word(c, V) + e, 8
+// consecutive values a load.  The loads need no branch: the one that would reach past the row's end, and
+// those behind it, take the last 8 values instead.  What is no value, or one of a slot before, is NaN:
+// every comparison and maximum passes over it.
+template <int DT, int T, int C>
+struct Row {
+  typename ops::IO<DT>::Raw r[C];
+
+  static __device__ __forceinline__ int word(int c, int V) {
+    return min(8 * ((int)threadIdx.x + T * c), max(V - 8, 0));
+  }
+  __device__ __forceinline__ void load(const void* base, int64_t at, int V) {
+    const float none = __builtin_nanf("");
+    if (V < 8) {  // shorter than a load: the first thread's first slots
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = threadIdx.x == 0 && e < V ? ops::IO<DT>::load1(base, at + e) : none;
+      put(0, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = none;
+#pragma unroll
+      for (int c = 1; c < C; ++c) put(c, v);
+      return;
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) r[c] = ops::load8_any<DT>(base, at + word(c, V));
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int first = 8 * ((int)threadIdx.x + T * c) - word(c, V);
+      if (first > 0) {
+        float v[8];
+        ops::IO<DT>::unpack(r[c], v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e >= first ? v[e] : none;
+        put(c, v);
+      }
+    }
+  }
+  // the 8 values of a load.  Each pass unpacks for itself: kept from pass to pass the values would take
+  // twice the registers of the row.
+  __device__ __forceinline__ void get(int c, float (&v)[8]) const {
+    typename ops::IO<DT>::Raw y = r[c];
+    asm volatile("" : "+v"(y.w[0]));
+    if constexpr (DT == ops::kDtFP32) asm volatile("" : "+v"(y.w[1]));
+    ops::IO<DT>::unpack(y, v);
+  }
+  // f(value, slot) over the slots
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float v[8];
+      get(c, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f(v[e], 8 * c + e);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+
+ private:
+  __device__ __forceinline__ void put(int c, const float* v) {
+    if constexpr (DT == ops::kDtFP32) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[c].w[e / 4][e % 4] = __float_as_uint(v[e]);
+    } else {
+      using E = typename std::conditional<DT == ops::kDtBF16, BF16, FP16>::type;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[c].w[0][e] = pack2<E>(v[2 * e], v[2 * e + 1]);  // exact
+    }
+  }
+};
+
+// The key of the k-th largest value: the largest t with count(key >= t) >= k.
+template <int DT, int T, int C>
+__device__ __forceinline__ uint32_t kth_key(const Row<DT, T, C>& x, int k, float* buf) {
+  uint32_t t = 0u;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t cand = t | (1u << bit);
+    float n = 0.f;
+    x.each([&](float v, int) { n += v == v && sample_key(v + 0.f) >= cand ? 1.f : 0.f; });
+    if (reduce_all<T, false>(n, buf) >= (float)k) t = cand;
+  }
+  return t;
+}
+
+// A row's RowTop, the same on every thread; one with a list has it in s.key / s.idx
+// (ordered by thread and slot), behind a barrier.
+//
+// The values that count are those >= t, t below the k-th largest and at least max - 110, where
+// an exponential is 0.  k <= T: every wave finds the ceil(k / waves)-th and the k-th
+// largest of its lanes' maxima, a ballot a bit; at least k values are >= the smallest
+// of the former and >= the largest of the latter.  About twice k random values pass; in
+// LDS, a value that fewer than k of them exceed is kept: ties of the k-th stay.  k > T:
+// the k-th largest itself, bit by bit with block-wide counts.
+template <int DT, int T, int C>
+__device__ __forceinline__ RowTop row_top(const void* base, int64_t row, int V, int k, RowLds<T>& s) {
+  constexpr int W = T / 64;
+  Row<DT, T, C> x;
+  x.load(base, row, V);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  float m = -INFINITY;
+  x.each([&](float v, int) { m = fmaxf(m, v); });
   uint32_t t1 = 0u, t2 = 0u;
-  if (list) {
-    const int k1 = (k + kSampleWaves - 1) / kSampleWaves;
+  if (k <= T && k < V) {
+    const uint32_t mx = sample_key(m + 0.f);
+    const int k1 = (k + W - 1) / W;
     for (int bit = 31; bit >= 0; --bit) {
       const uint32_t c1 = t1 | (1u << bit), c2 = t2 | (1u << bit);
       if (__popcll(__ballot(mx >= c1)) >= k1) t1 = c1;
       if (__popcll(__ballot(mx >= c2)) >= k) t2 = c2;
     }
   }
-  const float wmax = wave_reduce<0, true>(mx ? sample_unkey(mx) : -INFINITY);
+  const float wmax = wave_reduce<0, true>(m);
   if (lane == 0) {
     s.bound[0][wave] = t1;
     s.bound[1][wave] = t2;
@@ -101,43 +212,63 @@ __device__ __forceinline__ RowTop row_top(const uint32_t (&key)[EPT], int V, int
   }
   if (tid == 0) s.kth = 0xffffffffu;
   __syncthreads();
-  RowTop r{0u, s.top[0], 0.f, 0};
+  float top = s.top[0];
 #pragma unroll
-  for (int w = 0; w < kSampleWaves; ++w) {
-    r.max = fmaxf(r.max, s.top[w]);
+  for (int w = 0; w < W; ++w) {
+    top = fmaxf(top, s.top[w]);
     t1 = min(t1, s.bound[0][w]);
     t2 = max(t2, s.bound[1][w]);
   }
-  if (list) {
-    const uint32_t t = max(max(t1, t2), 1u);  // a key of 0 is no value
-    int mine = 0;
+  RowTop r{0u, fminf(top, __FLT_MAX__), 0.f, 0};
+  if (!(top > -__FLT_MAX__)) {  // nothing above the lowest float: all words alike
+    r.max = -__FLT_MAX__;
+    r.sum = (float)V;
+    return r;
+  }
+  r.kth = sample_key(r.max - 110.f + 0.f);
+  if (k < V) r.kth = max(r.kth, k <= T ? max(t1, t2) : kth_key(x, k, s.buf));
+  const float t = sample_unkey(r.kth);
+  uint32_t in[(C + 3) / 4] = {};  // the slots that count, 32 a word, the first in the highest bit
+  x.each([&](float v, int j) { in[j / 32] += in[j / 32] + (v >= t ? 1u : 0u); });
+  int mine = 0;
 #pragma unroll
-    for (int j = 0; j < EPT; ++j) mine += __popcll(__ballot(key[j] >= t));
-    if (lane == 0) s.count[wave] = mine;
-    __syncthreads();
-    int at = 0, n = 0;
+  for (int w = 0; w < (C + 3) / 4; ++w) mine += __popc(in[w]);
+  int upto = mine;  // of the wave's threads up to this one
 #pragma unroll
-    for (int w = 0; w < kSampleWaves; ++w) {
-      const int c = s.count[w];
-      at += w < wave ? c : 0;
-      n += c;
-    }
-    if (n <= kSampleCand) {
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += y;
+  }
+  if (lane == 63) s.count[wave] = upto;
+  __syncthreads();
+  int at = upto - mine, n = 0;
 #pragma unroll
-      for (int j = 0; j < EPT; ++j) {
-        const uint64_t mask = __ballot(key[j] >= t);
-        if (key[j] >= t) {
-          const int slot = at + __popcll(mask & ((1ull << lane) - 1));
-          s.key[slot] = key[j];
-          s.idx[slot] = tid + j * kSampleThreads;
+  for (int w = 0; w < W; ++w) {
+    const int c = s.count[w];
+    at += w < wave ? c : 0;
+    n += c;
+  }
+  if (n <= kVerifyList) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const uint32_t bits = in[c / 4] >> (8 * (min(C, 4) - 1 - c % 4)) & 255u;
+      if (!bits) continue;  // few threads have any
+      float v[8];
+      x.get(c, v);
+      const int word = Row<DT, T, C>::word(c, V);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (bits >> (7 - e) & 1u) {
+          s.key[at] = sample_key(fminf(v[e], __FLT_MAX__) + 0.f);
+          s.idx[at++] = word + e;
         }
-        at += __popcll(mask);
-      }
-      const int pad = n + tid;  // up to three zero keys complete the last group of four
-      if (tid < 3 && pad < kSampleCand) s.key[pad] = 0u;
-      __syncthreads();
-      const uint32_t own = tid < n ? s.key[tid] : 0u;
-      if (tid < n) {
+    }
+    const int pad = n + tid;  // up to three zero keys complete the last group of four
+    if (tid < 3 && pad < kVerifyList) s.key[pad] = 0u;
+    __syncthreads();
+    if (k < V && k <= T) {
+      for (int i = tid; i < n; i += T) {
+        const uint32_t own = s.key[i];
         int larger = 0;
         for (int c = 0; c < n; c += 4) {
           const u32x4 q = *reinterpret_cast<const u32x4*>(&s.key[c]);
@@ -148,70 +279,66 @@ __device__ __forceinline__ RowTop row_top(const uint32_t (&key)[EPT], int V, int
       }
       __syncthreads();
       r.kth = s.kth;
-      r.listed = n;
-      r.sum = block_reduce<false>(own >= r.kth ? expf(sample_unkey(own) - r.max) : 0.f, s.buf);
-      return r;
     }
+    float sum = 0.f;  // every wave for itself: the list is short
+    for (int i = lane; i < n; i += 64)
+      if (s.key[i] >= r.kth) sum += expf(sample_unkey(s.key[i]) - r.max);
+    r.sum = wave_reduce<0, false>(sum);
+    r.listed = n;
+    return r;
   }
-  if (k < V) {  // the largest t with count(key >= t) >= k, bit by bit
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t cand = r.kth | (1u << bit);
-      float c = 0.f;
-#pragma unroll
-      for (int j = 0; j < EPT; ++j) c += key[j] >= cand ? 1.f : 0.f;
-      if (block_reduce<false>(c, s.buf) >= (float)k) r.kth = cand;
-    }
-  } else {
-    r.kth = 1u;
+  // more values than the list holds: with k <= T the bound may lie below the k-th largest
+  if (k < V && k <= T) {
+    Row<DT, T, C> again;  // not kept in registers until here
+    asm volatile("" : "+s"(base));
+    again.load(base, row, V);
+    r.kth = max(r.kth, kth_key(again, k, s.buf));
   }
   float sum = 0.f;
-#pragma unroll
-  for (int j = 0; j < EPT; ++j)
-    if (key[j] >= r.kth) sum += expf(sample_unkey(key[j]) - r.max);
-  r.sum = block_reduce<false>(sum, s.buf);
+  for (int i = tid; i < V; i += T) {
+    const float v = load_logit<DT>(base, row + i);
+    if (sample_key(v) >= r.kth) sum += expf(v - r.max);
+  }
+  r.sum = reduce_all<T, false>(sum, s.buf);
   return r;
 }
 
-// One row a workgroup: blockIdx.x = (drafter?, b, n).
-template <int DT, int EPT>
-__global__ __launch_bounds__(kSampleThreads) void verify_rows_kernel(VerifyParams p) {
-  __shared__ RowLds s;
+// One row a workgroup: blockIdx.x = (drafter?, b, n) with n < ahead.
+template <int DT, int T, int C>
+__global__ __launch_bounds__(T) void verify_rows_kernel(VerifyParams p) {
+  __shared__ RowLds<T> s;
   const int tid = threadIdx.x, lane = tid & 63;
-  const int w = blockIdx.x >= p.B * p.N, row = blockIdx.x - w * p.B * p.N, b = row / p.N, n = row % p.N;
+  const int rows = p.B * p.ahead, w = blockIdx.x >= rows, row = blockIdx.x - w * rows, b = row / p.ahead, n = row % p.ahead;
   // a row that no walk can reach or use: of padding, and a drafter's without children
   if (w) {
     if (!__ballot(lane < p.N && lane > n && verify_parent(p, b, lane < p.N ? lane : 0) == n)) return;
   } else if (verify_parent(p, b, n) < -1) {
     return;
   }
-  uint32_t key[EPT];
-  const int64_t at = b * p.s[w][0] + n * p.s[w][1];
-#pragma unroll
-  for (int j = 0; j < EPT; ++j) {
-    const int i = tid + j * kSampleThreads;
-    key[j] = i < p.V ? sample_key(load_logit<DT>(p.rows[w], at + i)) : 0u;
-  }
-  const RowTop r = row_top<EPT>(key, p.V, p.k, s);
+  const RowTop r = row_top<DT, T, C>(p.rows[w], b * p.s[w][0] + n * p.s[w][1], p.V, p.k, s);
   if (tid == 0) p.top[blockIdx.x] = r;
-  if (!w && tid < r.listed) p.list[(int64_t)row * kSampleCand + tid] = u32x2{s.key[tid], (uint32_t)s.idx[tid]};
+  if (!w)
+    for (int i = tid; i < r.listed; i += T) p.list[(int64_t)row * kVerifyList + i] = u32x2{s.key[i], (uint32_t)s.idx[i]};
 }
 
 // A walk: LDS copies of what every node's test needs, and the node's rejections.
+template <int T>
 struct WalkLds {
   RowTop top[2][kTreeNodes];
   int parents[kTreeNodes], path[kTreeNodes];
   int64_t tokens[kTreeNodes];
   float uniform[kTreeNodes];
   float logit[2][kTreeNodes];  // of a node's token in its parent's rows
-  float sums[kTreeNodes];      // W of p before each rejection (drafter), else:
-  int64_t gone[kTreeNodes];    // the rejected tokens
-  float buf[kSampleWaves];
-  unsigned long long best[kSampleWaves];
+  float sums[kTreeNodes];      // W of p before each rejection,
+  int64_t gone[kTreeNodes];    // and the rejected tokens
+  float buf[T / 64];
+  unsigned long long best[T / 64];
+  RowLds<T> row;  // of a node past the rows taken ahead
 };
 
-template <int DT, bool DRAFT>
-__global__ __launch_bounds__(kSampleThreads) void verify_walk_kernel(VerifyParams p) {
-  __shared__ WalkLds s;
+template <int DT, int T, int C, bool DRAFT>
+__global__ __launch_bounds__(T) void verify_walk_kernel(VerifyParams p) {
+  __shared__ WalkLds<T> s;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, N = p.N;
   if (tid < N) {
     const int up = verify_parent(p, b, tid);
@@ -223,7 +350,7 @@ __global__ __launch_bounds__(kSampleThreads) void verify_walk_kernel(VerifyParam
     const bool asked = up >= 0 && x >= 0 && x < p.V;
 #pragma unroll
     for (int w = 0; w <= (DRAFT ? 1 : 0); ++w) {
-      s.top[w][tid] = p.top[(int64_t)w * p.B * N + (int64_t)b * N + tid];
+      if (tid < p.ahead) s.top[w][tid] = p.top[((int64_t)w * p.B + b) * p.ahead + tid];
       // a token outside the vocabulary has probability 0
       s.logit[w][tid] = asked ? load_logit<DT>(p.rows[w], b * p.s[w][0] + up * p.s[w][1] + x) : -INFINITY;
     }
@@ -236,9 +363,22 @@ __global__ __launch_bounds__(kSampleThreads) void verify_walk_kernel(VerifyParam
     if (tid == 0) s.path[count] = here;
     ++count;
     uint64_t kids = __ballot(lane < N && s.parents[lane < N ? lane : 0] == here);
-    const RowTop tp = s.top[0][here], tq = s.top[DRAFT ? 1 : 0][here];
     const int64_t xat = b * p.s[0][0] + here * p.s[0][1], yat = DRAFT ? b * p.s[1][0] + here * p.s[1][1] : 0;
-    const u32x2* list = p.list + ((int64_t)b * N + here) * kSampleCand;
+    const bool ready = here < p.ahead;
+    RowTop tp, tq{};
+    if (ready) {
+      tp = s.top[0][here];
+      if constexpr (DRAFT) tq = s.top[1][here];
+    } else {
+      if constexpr (DRAFT)
+        if (kids) {
+          __syncthreads();  // the last reads of the row's LDS are done
+          tq = row_top<DT, T, C>(p.rows[1], yat, p.V, p.k, s.row);
+        }
+      __syncthreads();
+      tp = row_top<DT, T, C>(p.rows[0], xat, p.V, p.k, s.row);
+    }
+    const u32x2* list = p.list + ((int64_t)b * p.ahead + here) * kVerifyList;
     const int n = tp.listed ? tp.listed : p.V;
     float W = tp.sum;
     int gone = 0;  // rejections that changed p
@@ -248,23 +388,37 @@ __global__ __launch_bounds__(kSampleThreads) void verify_walk_kernel(VerifyParam
         w = DRAFT ? fmaxf(w * (1.f / s.sums[j]) - q, 0.f) : word == s.gone[j] ? 0.f : w;
       return w;
     };
-    // f(weight, q, word) over the words of this thread
+    // a word of the node: its index, its kept exponential (0: none) and the drafter's probability
+    struct Entry {
+      int word;
+      float w, q;
+    };
+    const bool asks = kids != 0;
+    auto entry = [&](int i) {
+      Entry e{i, 0.f, 0.f};
+      if (i >= n) return e;
+      if (tp.listed) {
+        const u32x2 x = ready ? list[i] : u32x2{s.row.key[i], (uint32_t)s.row.idx[i]};
+        e.word = (int)x[1];
+        e.w = x[0] >= tp.kth ? expf(sample_unkey(x[0]) - tp.max) : 0.f;
+      } else {
+        e.w = kept(load_logit<DT>(p.rows[0], xat + i), tp);
+      }
+      if constexpr (DRAFT)
+        if (asks && e.w > 0.f) e.q = kept(load_logit<DT>(p.rows[1], yat + e.word), tq) * (1.f / tq.sum);
+      return e;
+    };
+    // f(weight, q, word) over the words of this thread.  Its first is loaded once a node, when a rejection or
+    // the draw first needs it: lists are mostly shorter than the workgroup.
+    Entry own;
+    bool loaded = false;
     auto each = [&](auto f) {
-      for (int i = tid; i < n; i += kSampleThreads) {
-        int word = i;
-        float w;
-        if (tp.listed) {
-          const u32x2 e = list[i];
-          word = (int)e[1];
-          w = e[0] >= tp.kth ? expf(sample_unkey(e[0]) - tp.max) : 0.f;
-        } else {
-          w = kept(load_logit<DT>(p.rows[0], xat + i), tp);
-        }
-        if (!(w > 0.f)) continue;
-        float q = 0.f;
-        if constexpr (DRAFT)
-          if (gone || kids) q = kept(load_logit<DT>(p.rows[1], yat + word), tq) * (1.f / tq.sum);
-        f(weight(w, q, word), q, word);
+      if (!loaded) own = entry(tid);
+      loaded = true;
+      if (own.w > 0.f) f(weight(own.w, own.q, own.word), own.q, own.word);
+      for (int i = tid + T; i < n; i += T) {
+        const Entry e = entry(i);
+        if (e.w > 0.f) f(weight(e.w, e.q, e.word), e.q, e.word);
       }
     };
     int next = -1;
@@ -280,7 +434,7 @@ __global__ __launch_bounds__(kSampleThreads) void verify_walk_kernel(VerifyParam
       float sum = 0.f;
       const float inv = 1.f / W;
       each([&](float w, float qw, int word) { sum += DRAFT ? fmaxf(w * inv - qw, 0.f) : word == x ? 0.f : w; });
-      sum = block_reduce<false>(sum, s.buf);
+      sum = reduce_all<T, false>(sum, s.buf);
       if (sum > 0.f) {
         if (tid == 0) {
           s.sums[gone] = W;
@@ -311,7 +465,7 @@ __global__ __launch_bounds__(kSampleThreads) void verify_walk_kernel(VerifyParam
     if (lane == 0) s.best[tid >> 6] = best;
     __syncthreads();
 #pragma unroll
-    for (int v = 0; v < kSampleWaves; ++v) best = s.best[v] > best ? s.best[v] : best;
+    for (int v = 0; v < T / 64; ++v) best = s.best[v] > best ? s.best[v] : best;
     if (best) drawn = (int64_t)(0xffffffffu - (uint32_t)best);
   }
   __syncthreads();
