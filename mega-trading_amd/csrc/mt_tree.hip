@@ -43,6 +43,8 @@ int check_rows16(const char* name, const void* p, const int64_t* s) {
     if (s[i] < 0 || s[i] % 8)
       return fail(MT_E_STRIDE, "%s: stride %d (%lld) must be a non-negative multiple of 8 elements", name, i,
                   (long long)s[i]);
+  // the copies keep 16 rows of offsets in 32-bit registers
+  if (s[2] > (int64_t(1) << 24)) return fail(MT_E_STRIDE, "%s: row stride %lld too large", name, (long long)s[2]);
   return MT_OK;
 }
 
@@ -80,31 +82,47 @@ mt::TreeShape shape(const int* parents, int64_t parents_stride, const int* lengt
   return t;
 }
 
-// Query rows of a workgroup (32 NT), row blocks of a KV head and workgroups its keys are split over.
+// The attention's launch: row waves of a workgroup (RW, 0 for the few-row kernel), row blocks of a KV
+// head and workgroups its keys are split over.
 struct Split {
-  int nt, blocks;
+  int rw, blocks, keys, groups;
   int64_t nspan;
 };
-Split split(int64_t B, int64_t Hkv, int64_t R, int N, int64_t keys, int D) {
+Split split(int64_t B, int64_t Hkv, int64_t R, int N, int64_t cached, int D) {
   Split s;
   const int64_t rows = R * N;
-  s.nt = rows <= 32 ? 1 : 2;
-  s.blocks = (int)((rows + 32 * s.nt - 1) / (32 * s.nt));
-  const int64_t tiles = (keys + mt::kTreeKeys - 1) / mt::kTreeKeys + (N + mt::kTreeKeys - 1) / mt::kTreeKeys;
-  const int64_t want = (D == 128 ? 2 : 4) * (int64_t)device_cus() / std::max<int64_t>(1, B * Hkv * s.blocks);
-  const int64_t most = (tiles + 2 * mt::kTreeWaves - 1) / (2 * mt::kTreeWaves);  // two tiles a wave
+  s.rw = rows <= 32 ? 0 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
+  const int take = s.rw ? 32 * s.rw : 32, waves = D == 128 ? 8 : 16;
+  s.keys = s.rw ? 16 * s.rw : mt::kTreeKeys;
+  s.groups = s.rw ? waves / s.rw : waves / 2;
+  s.blocks = (int)((rows + take - 1) / take);
+  const int64_t tiles = (cached + s.keys - 1) / s.keys + (N + s.keys - 1) / s.keys;
+  // A workgroup fills a CU.  Up to 192 keys a key group stay with one workgroup: joining spans is another
+  // launch (5 nodes on 200 of 1024 cached keys, 2 heads of 64: 6.5 us against 7.0 and 3.4; 16 nodes, 32 sequences
+  // of about 500: 12.9 against 11.9 and 3.5; 64 nodes there, 2 key groups: 26.0 against 20.6 and 5.5).  More are split over all
+  // CUs, down to two tiles.
+  const int64_t want = (int64_t)device_cus() / std::max<int64_t>(1, B * Hkv * s.blocks);
+  const int64_t most = tiles * s.keys <= 192 * s.groups ? 1 : (tiles + 2 * s.groups - 1) / (2 * s.groups);
   s.nspan = std::max<int64_t>(1, std::min(want, most));
   return s;
 }
 
 template <class E, int D>
-void launch_tree(const mt::TreeAttnParams& p, int nt, unsigned grid, hipStream_t st) {
-  if (nt == 1) hipLaunchKernelGGL((mt::tree_attn_kernel<E, D, 1>), dim3(grid), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((mt::tree_attn_kernel<E, D, 2>), dim3(grid), dim3(256), 0, st, p);
-  if (p.nspan > 1) {
-    const int64_t n = (int64_t)p.B * p.Hkv * p.R * p.t.N * (D / 4);
-    hipLaunchKernelGGL((mt::tree_combine_kernel<E, D>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, p);
-  }
+void launch_tree(const mt::TreeAttnParams& p, int rw, unsigned grid, hipStream_t st) {
+  const dim3 few(64 * mt::tree_few_waves<D>()), many(64 * mt::tree_waves<D>());
+  if (rw == 0) hipLaunchKernelGGL((mt::tree_attn_kernel<E, D>), dim3(grid), few, 0, st, p);
+  else if (rw == 2) hipLaunchKernelGGL((mt::tree_attn_rows_kernel<E, D, 2>), dim3(grid), many, 0, st, p);
+  else if (rw == 4) hipLaunchKernelGGL((mt::tree_attn_rows_kernel<E, D, 4>), dim3(grid), many, 0, st, p);
+  else hipLaunchKernelGGL((mt::tree_attn_rows_kernel<E, D, 8>), dim3(grid), many, 0, st, p);
+  if (p.nspan == 1) return;
+  // up to 8 spans come in one batch of loads, and threads that share a row would only add their meeting
+  // (2 spans, 49152 rows of 128: 6.8 / 17.5 us; 118 spans, 512 rows of 64: 10.3 / 4.5)
+  const int64_t n = (int64_t)p.B * p.Hkv * p.R * p.t.N, few_rows = 256 / (D / 4), many_rows = few_rows / 8;
+  if (p.nspan <= 8)
+    hipLaunchKernelGGL((mt::tree_combine_kernel<E, D, 1>), dim3((unsigned)((n + few_rows - 1) / few_rows)), dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((mt::tree_combine_kernel<E, D, 8>), dim3((unsigned)((n + many_rows - 1) / many_rows)), dim3(256), 0,
+                       st, p);
 }
 
 // Nodes of a sequence whose rows are taken before the walk: as many as the card works on at a time.
@@ -259,21 +277,23 @@ int mt_tree_attn(const void* q, const void* k, const void* v, const void* k_cach
   p.R = Hq / Hkv;
   p.nspan = (int)s.nspan;
   p.blocks = s.blocks;
+  p.keys = s.keys;
+  p.groups = s.groups;
   p.scale_log2 = scale * mt::kLog2e;
   const int64_t groups = ((int64_t)B * Hkv * s.nspan + 7) / 8 * 8;
   const int64_t rows = (int64_t)B * Hq * N;
-  if (groups * s.blocks > 0x7fffffffLL || rows * (D / 4) > 0x7fffffffLL * 256)
+  if (groups * s.blocks > 0x7fffffffLL || rows > 0x7fffffffLL)
     return fail(MT_E_SHAPE, "too many query rows (%lld)", (long long)rows);
   const unsigned grid = (unsigned)(groups * s.blocks);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == MT_DTYPE_BF16) {
-    if (D == 32) launch_tree<mt::BF16, 32>(p, s.nt, grid, st);
-    else if (D == 64) launch_tree<mt::BF16, 64>(p, s.nt, grid, st);
-    else launch_tree<mt::BF16, 128>(p, s.nt, grid, st);
+    if (D == 32) launch_tree<mt::BF16, 32>(p, s.rw, grid, st);
+    else if (D == 64) launch_tree<mt::BF16, 64>(p, s.rw, grid, st);
+    else launch_tree<mt::BF16, 128>(p, s.rw, grid, st);
   } else {
-    if (D == 32) launch_tree<mt::FP16, 32>(p, s.nt, grid, st);
-    else if (D == 64) launch_tree<mt::FP16, 64>(p, s.nt, grid, st);
-    else launch_tree<mt::FP16, 128>(p, s.nt, grid, st);
+    if (D == 32) launch_tree<mt::FP16, 32>(p, s.rw, grid, st);
+    else if (D == 64) launch_tree<mt::FP16, 64>(p, s.rw, grid, st);
+    else launch_tree<mt::FP16, 128>(p, s.rw, grid, st);
   }
   return launched("tree attention");
 }

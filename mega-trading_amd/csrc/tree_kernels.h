@@ -128,20 +128,22 @@ struct TreeAttnParams {
   int B, Hkv, R;
   int nspan;   // workgroups a row block's keys are split over
   int blocks;  // row blocks of a KV head
+  int keys, groups;  // of a tile, and key groups of a workgroup
   float scale_log2;
 };
 
 constexpr int kTreeKeys = 32;   // keys of a wave's tile
-constexpr int kTreeWaves = 4;
 constexpr float kTreeNone = -1e30f;  // offset of a row that has seen no key: finite, so nothing of it turns into NaN
 
-// Tiles of 32 keys: the prefix's, then the tree's; and how many of them a wave takes.
+// Key tiles: the prefix's, then the tree's; and how many of them each of the `groups` key groups of a
+// span takes.
 struct TreeTiles {
-  int prefix, all, per;
-  __device__ __forceinline__ TreeTiles(int cached, int N, int nspan) {
-    prefix = (cached + kTreeKeys - 1) / kTreeKeys;
-    all = prefix + (N + kTreeKeys - 1) / kTreeKeys;
-    per = (all + kTreeWaves * nspan - 1) / (kTreeWaves * nspan);
+  int prefix, all, per, spans;
+  __device__ __forceinline__ TreeTiles(int cached, int N, int nspan, int keys, int groups) {
+    prefix = (cached + keys - 1) / keys;
+    all = prefix + (N + keys - 1) / keys;
+    per = (all + groups * nspan - 1) / (groups * nspan);
+    spans = (all + groups * per - 1) / (groups * per);  // that hold tiles
   }
 };
 
@@ -157,15 +159,48 @@ __device__ __forceinline__ void copy_rows32(char* lds, const uint16_t* src, int6
   }
 }
 
-template <class E, int D, int NT>
-__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void tree_attn_kernel(TreeAttnParams p) {
+// Four values (chunk c) of a query row from the W key groups of a workgroup: M = max m_w,
+// o = sum_w 2^(m_w - M) o_w, l the same sum of l_w; into the output, or this span's partial.
+template <class E, int D, int W, class FM, class FL, class FO>
+__device__ __forceinline__ void tree_merge(const TreeAttnParams& p, int pair, int s, int row, int c, FM m, FL l, FO x) {
+  const int64_t at = (int64_t)pair * p.R * p.t.N + row;
+  float M = m(0), lt = 0.f;
+#pragma unroll
+  for (int w = 1; w < W; ++w) M = fmaxf(M, m(w));
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const float a = exp2_fast(m(w) - M);
+    const f32x4 y = x(w);
+    lt = __builtin_fmaf(a, l(w), lt);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(a, y[e], o[e]);
+  }
+  if (p.nspan == 1) {
+    const float inv = 1.f / lt;
+    u32x2 y = {pack2<E>(o[0] * inv, o[1] * inv), pack2<E>(o[2] * inv, o[3] * inv)};
+    if (lt == 0.f) y = u32x2{0u, 0u};
+    *reinterpret_cast<u32x2*>(p.out + at * D + 4 * c) = y;
+  } else {
+    float* dst = p.part + (at * p.nspan + s) * (D + 4);
+    *reinterpret_cast<f32x4*>(dst + 4 * c) = o;
+    if (c == 0) *reinterpret_cast<f32x2*>(dst + D) = f32x2{M, lt};
+  }
+}
+
+template <int D>
+constexpr int tree_few_waves() { return D == 128 ? 4 : 8; }  // what the tiles leave room for: one workgroup a CU
+
+template <class E, int D>
+__global__ __launch_bounds__(64 * tree_few_waves<D>()) void tree_attn_kernel(TreeAttnParams p) {
+  constexpr int NT = 1, W = tree_few_waves<D>();
   using V8 = typename E::v8;
   using TL = Tile<D>;
   constexpr int KT = D / 16, DT = D / 32, TILE = kTreeKeys * TL::RB;
   constexpr int COPIES = 2 * TILE / 1024;  // of a K and a V tile
   constexpr int C4 = D / 4;                // 16-byte chunks of an fp32 row
-  __shared__ __attribute__((aligned(1024))) char smem[kTreeWaves][2][2][TILE];  // then the waves' o [32 NT][D] fp32
-  __shared__ float wm[kTreeWaves][32 * NT], wl[kTreeWaves][32 * NT];
+  __shared__ __attribute__((aligned(1024))) char smem[W][2][2][TILE];  // then the waves' o [32 NT][D] fp32
+  __shared__ float wm[W][32 * NT], wl[W][32 * NT];
   static_assert(sizeof(smem[0]) >= 32 * NT * D * 4, "a wave's o fits its tiles");
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -174,9 +209,9 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void tree_attn_kernel(TreeAt
   if (g >= p.B * p.Hkv * p.nspan) return;
   const int s = g % p.nspan, pair = g / p.nspan, kvh = pair % p.Hkv, b = pair / p.Hkv;
   const int L = p.t.cached(b), N = p.t.N, RN = p.R * N;
-  const TreeTiles tl(L, N, p.nspan);
-  if (s * kTreeWaves * tl.per >= tl.all) return;  // the combine does not read this span
-  const int t0 = (s * kTreeWaves + wave) * tl.per, t1 = min(tl.all, t0 + tl.per);
+  const TreeTiles tl(L, N, p.nspan, kTreeKeys, W);
+  if (s >= tl.spans) return;  // the combine does not read this span
+  const int t0 = (s * W + wave) * tl.per, t1 = min(tl.all, t0 + tl.per);
 
   const uint16_t* kc = p.kc + b * p.skc[0] + (int64_t)kvh * p.skc[1];
   const uint16_t* vc = p.vc + b * p.svc[0] + (int64_t)kvh * p.svc[1];
@@ -340,79 +375,257 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void tree_attn_kernel(TreeAt
       }
   }
   __syncthreads();
-  for (int i = tid; i < 32 * NT * C4; i += 64 * kTreeWaves) {
+  for (int i = tid; i < 32 * NT * C4; i += 64 * W) {
     const int r = i / C4, c = i % C4, row = rb * NT * 32 + r;
     if (row >= RN) continue;
-    float M = wm[0][r], lt = 0.f;
-#pragma unroll
-    for (int w = 1; w < kTreeWaves; ++w) M = fmaxf(M, wm[w][r]);
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < kTreeWaves; ++w) {
-      const float a = exp2_fast(wm[w][r] - M);
-      const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(smem[w]) + r * D + 4 * (c ^ (r % C4)));
-      lt = __builtin_fmaf(a, wl[w][r], lt);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(a, x[e], o[e]);
-    }
-    if (p.nspan == 1) {
-      const float inv = 1.f / lt;
-      u32x2 y = {pack2<E>(o[0] * inv, o[1] * inv), pack2<E>(o[2] * inv, o[3] * inv)};
-      if (lt == 0.f) y = u32x2{0u, 0u};
-      *reinterpret_cast<u32x2*>(p.out + (((int64_t)b * p.Hkv + kvh) * RN + row) * D + 4 * c) = y;
-    } else {
-      float* dst = p.part + (((int64_t)pair * RN + row) * p.nspan + s) * (D + 4);
-      *reinterpret_cast<f32x4*>(dst + 4 * c) = o;
-      if (c == 0) *reinterpret_cast<f32x2*>(dst + D) = f32x2{M, lt};
-    }
+    tree_merge<E, D, W>(p, pair, s, row, c, [&](int w) { return wm[w][r]; }, [&](int w) { return wl[w][r]; },
+                                 [&](int w) {
+                                   return *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(smem[w]) + r * D +
+                                                                          4 * (c ^ (r % C4)));
+                                 });
   }
 }
 
-// Joins the spans of each query row: M = max m_s, o = sum_s 2^(m_s - M) o_s over the
-// same sum of l_s.  One thread per 4 values of a row, 8 spans in flight.
-template <class E, int D>
+// Many query rows: W waves of 32 rows, RW of them on one key tile of 16 RW keys, so that a tile in
+// LDS feeds up to 32 RW rows; W / RW key groups, 16 W keys a step in all.  Two buffers; every wave copies 16 rows
+// of its group's next tile while it works on the present one, and one barrier a step orders both.
+// Two waves a SIMD (four at D <= 64) let one's softmax run beside the other's products.
+template <int D>
+constexpr int tree_waves() { return D == 128 ? 8 : 16; }  // what the tiles leave room for: one workgroup a CU
+
+template <class E, int D, int RW>
+__global__ __launch_bounds__(64 * tree_waves<D>()) void tree_attn_rows_kernel(TreeAttnParams p) {
+  using V8 = typename E::v8;
+  using TL = Tile<D>;
+  constexpr int KT = D / 16, DT = D / 32, C4 = D / 4, W = tree_waves<D>();
+  constexpr int KEYS = 16 * RW, KW = W / RW, TILE = KEYS * TL::RB, NQ = KEYS / 32;
+  constexpr bool AHEAD = D == 128;  // a quarter's scores beside the last one's softmax; else other waves' are
+  __shared__ __attribute__((aligned(1024))) char smem[2][KW][2][TILE];  // then the waves' o [32][D] fp32
+  __shared__ float wm[W][32], wl[W][32];
+  static_assert(sizeof(smem) == W * 32 * D * 4, "the waves' o fill the tiles");
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kw = wave / RW, rw = wave % RW;
+  const int slot = blockIdx.x % (8 * p.blocks), g = blockIdx.x / (8 * p.blocks) * 8 + slot % 8, rb = slot / 8;
+  if (g >= p.B * p.Hkv * p.nspan) return;
+  const int s = g % p.nspan, pair = g / p.nspan, kvh = pair % p.Hkv, b = pair / p.Hkv;
+  const int L = p.t.cached(b), N = p.t.N, RN = p.R * N;
+  const TreeTiles tl(L, N, p.nspan, KEYS, KW);
+  if (s >= tl.spans) return;  // the combine does not read this span
+  const int steps = min(tl.per, (tl.all - s * KW * tl.per + KW - 1) / KW);
+  const int first = s * KW * tl.per + kw;  // the group's tiles: first + KW i
+
+  const uint16_t* kc = p.kc + b * p.skc[0] + (int64_t)kvh * p.skc[1];
+  const uint16_t* vc = p.vc + b * p.svc[0] + (int64_t)kvh * p.svc[1];
+  const uint16_t* kn = p.k + b * p.sk[0] + (int64_t)kvh * p.sk[1];
+  const uint16_t* vn = p.v + b * p.sv[0] + (int64_t)kvh * p.sv[1];
+  const uint64_t anc = tree_ancestors(p.t, b, lane);
+  const uint64_t padding = ~__ballot(anc != 0ull);
+  WaveStager<uint16_t, D, 16> ks, vs;
+  ks.init(p.skc[2], lane);
+  vs.init(p.svc[2], lane);
+  // the wave's 16 rows of its group's tile t
+  auto stage = [&](int t, int buf) {
+    if (t >= tl.all) return;
+    char *kl = smem[buf][kw][0] + rw * 16 * TL::RB, *vl = smem[buf][kw][1] + rw * 16 * TL::RB;
+    if (t < tl.prefix) {
+      ks.stage(kl, kc, p.skc[2], t * KEYS + rw * 16, L);
+      vs.stage(vl, vc, p.svc[2], t * KEYS + rw * 16, L);
+    } else {
+      // the tree's, through registers: what padding holds is replaced by zeros, since 0 times it must be 0
+      const int n0 = (t - tl.prefix) * KEYS + rw * 16;
+#pragma unroll
+      for (int i = 0; i < TL::NC / 4; ++i) {
+        const int f = i * 64 + lane, row = f / TL::NC, chunk = (f % TL::NC) ^ TL::swz(row), n = n0 + row;
+        const bool in = n < N && !(padding >> (n & 63) & 1);
+        const u32x4 a = *reinterpret_cast<const u32x4*>(kn + (int64_t)min(n, N - 1) * p.sk[2] + chunk * 8);
+        const u32x4 c = *reinterpret_cast<const u32x4*>(vn + (int64_t)min(n, N - 1) * p.sv[2] + chunk * 8);
+        *reinterpret_cast<u32x4*>(kl + f * 16) = in ? a : zero4();
+        *reinterpret_cast<u32x4*>(vl + f * 16) = in ? c : zero4();
+      }
+    }
+  };
+  stage(first, 0);
+
+  const int row = (rb * RW + rw) * 32 + l32, rc = min(row, RN - 1), node = rc % N;
+  const bool active = (rb * RW + rw) * 32 < RN;  // wave-uniform
+  const uint64_t up = shfl64(anc, node), seen = row < RN ? up : 0ull;
+  V8 qop[KT];
+  {
+    const uint16_t* qr = p.q + b * p.sq[0] + (int64_t)(kvh * p.R + rc / N) * p.sq[1] + (int64_t)node * p.sq[2] + 8 * hh;
+#pragma unroll
+    for (int kk = 0; kk < KT; ++kk) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(qr + 16 * kk);
+      qop[kk] = __builtin_bit_cast(V8, seen ? x : zero4());
+    }
+  }
+  f32x16 oacc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) zero16(oacc[dt]);
+  float mrun = kTreeNone, lrun = 0.f;
+  const int rbase = TL::row_base(lane);
+  const TrBase tbase = TL::tr_base(lane);
+  const float c2 = p.scale_log2;
+
+  for (int i = 0; i < steps; ++i) {
+    const int t = first + KW * i, buf = i & 1;
+    wait_vmem();
+    __syncthreads();  // this step's tiles are there, and the last step's are read
+    if (i + 1 < steps) stage(t + KW, buf ^ 1);
+    if (!active || t >= tl.all) continue;
+    const char *kl = smem[buf][kw][0], *vl = smem[buf][kw][1];
+    const int n0 = (t - tl.prefix) * KEYS;  // the tile's first node, from 0 on
+    const bool mask = n0 >= 0 || (t + 1) * KEYS > L;
+    f32x16 st[AHEAD ? 2 : 1];
+    auto scores = [&](int h, f32x16& x) {
+#pragma unroll
+      for (int kk = 0; kk < KT; ++kk)
+        x = E::mfma(TL::template row_op<E>(kl, rbase, 32 * h, kk), qop[kk], kk == 0 ? f32x16{} : x);
+    };
+    if (AHEAD) scores(0, st[0]);
+#pragma unroll
+    for (int h = 0; h < NQ; ++h) {
+      f32x16& x = st[AHEAD ? h & 1 : 0];
+      if (!AHEAD) scores(h, x);
+      else if (h + 1 < NQ) scores(h + 1, st[(h + 1) & 1]);
+      if (mask) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int key = 32 * h + 8 * (j >> 2) + 4 * hh + (j & 3), n = n0 + key;
+          const bool in = n0 >= 0 ? n < 64 && (seen >> (n & 63) & 1) : t * KEYS + key < L;
+          x[j] = in ? x[j] : -INFINITY;
+        }
+      }
+      V8 pk[2];
+      float qs;
+      auto ex = [&]() {  // as in tree_attn_kernel
+        u32x4 w[2];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          w[j >> 2][j & 3] = pack2<E>(exp2_fast(__builtin_fmaf(x[2 * j], c2, -mrun)),
+                                      exp2_fast(__builtin_fmaf(x[2 * j + 1], c2, -mrun)));
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s0 = E::sum2(w[0][j], s0);
+          s1 = E::sum2(w[1][j], s1);
+        }
+        qs = s0 + s1;
+        pk[0] = __builtin_bit_cast(V8, w[0]);
+        pk[1] = __builtin_bit_cast(V8, w[1]);
+      };
+      ex();
+      if (__builtin_amdgcn_ballot_w64(!(qs <= kSumLimit))) {
+        float v = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v = fmaxf(v, x[j]);
+        const bool raise = max_with_partner(qs <= kSumLimit ? 0.f : 1.f) > 0.f;
+        v = max_with_partner(v) * c2;
+        const float m = raise ? fmaxf(mrun, v) : mrun, alpha = exp2_fast(mrun - m);
+        mrun = m;
+        lrun *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) oacc[dt][j] *= alpha;
+        ex();
+      }
+      lrun += qs;
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          oacc[dt] = E::mfma(TL::template tr_op<E>(vl, tbase, 2 * h + k2, dt), pk[k2], oacc[dt]);
+    }
+  }
+  __syncthreads();
+
+  float* ow = reinterpret_cast<float*>(&smem[0][0][0][0]) + wave * 32 * D;
+  {
+    const float l = sum_with_partner(lrun);
+    if (hh == 0) {
+      wm[wave][l32] = seen ? mrun : kTreeNone;
+      wl[wave][l32] = seen ? l : 0.f;
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = dt * 8 + 2 * q + hh;
+        *reinterpret_cast<f32x4*>(ow + l32 * D + 4 * (c ^ (l32 % C4))) =
+            f32x4{oacc[dt][4 * q], oacc[dt][4 * q + 1], oacc[dt][4 * q + 2], oacc[dt][4 * q + 3]};
+      }
+  }
+  __syncthreads();
+  for (int i = tid; i < 32 * RW * C4; i += 64 * W) {
+    const int r = i / C4, c = i % C4, l = r % 32, w0 = r / 32, at = rb * RW * 32 + r;
+    if (at >= RN) continue;
+    tree_merge<E, D, KW>(p, pair, s, at, c, [&](int w) { return wm[w * RW + w0][l]; },
+                         [&](int w) { return wl[w * RW + w0][l]; }, [&](int w) {
+                           return *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(&smem[0][0][0][0]) +
+                                                                  (w * RW + w0) * 32 * D + l * D + 4 * (c ^ (l % C4)));
+                         });
+  }
+}
+
+// Joins the spans of each query row: M = max m_s, o = sum_s 2^(m_s - M) o_s over the same sum of
+// l_s.  JOIN threads for each 4 values of a row share its spans, 8 of them in flight each, and meet in LDS.
+template <class E, int D, int JOIN>
 __global__ __launch_bounds__(256) void tree_combine_kernel(TreeAttnParams p) {
-  constexpr int C4 = D / 4, ROW = D + 4, BATCH = 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = i / C4;
-  const int c = i % C4, RN = p.R * p.t.N;
-  if (row >= (int64_t)p.B * p.Hkv * RN) return;
+  constexpr int C4 = D / 4, ROW = D + 4, BATCH = 8, ROWS = 256 / (C4 * JOIN);
+  __shared__ __attribute__((aligned(16))) float part[ROWS][JOIN][ROW];
+  const int tid = threadIdx.x, c = tid % C4, j = tid / C4 % JOIN, r = tid / (C4 * JOIN), RN = p.R * p.t.N;
+  const int64_t row = min((int64_t)blockIdx.x * ROWS + r, (int64_t)p.B * p.Hkv * RN - 1);  // the last ones twice
   const int b = int(row / ((int64_t)p.Hkv * RN));
-  const TreeTiles tl(p.t.cached(b), p.t.N, p.nspan);
-  const int ns = (tl.all + kTreeWaves * tl.per - 1) / (kTreeWaves * tl.per);  // spans that held keys
+  const int ns = TreeTiles(p.t.cached(b), p.t.N, p.nspan, p.keys, p.groups).spans;
   const float* src = p.part + row * p.nspan * ROW;
   float M = kTreeNone, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < ns; s0 += BATCH) {
+  for (int s0 = j; s0 < ns; s0 += BATCH * JOIN) {
     f32x2 ml[BATCH];
     f32x4 x[BATCH];
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j) {
-      const float* r = src + (int64_t)min(s0 + j, ns - 1) * ROW;
-      ml[j] = *reinterpret_cast<const f32x2*>(r + D);
-      x[j] = *reinterpret_cast<const f32x4*>(r + 4 * c);
+    for (int i = 0; i < BATCH; ++i) {
+      const float* q = src + (int64_t)min(s0 + JOIN * i, ns - 1) * ROW;
+      ml[i] = *reinterpret_cast<const f32x2*>(q + D);
+      x[i] = *reinterpret_cast<const f32x4*>(q + 4 * c);
     }
     float mn = M;
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j) mn = fmaxf(mn, ml[j][0]);
+    for (int i = 0; i < BATCH; ++i) mn = fmaxf(mn, ml[i][0]);
     const float a = exp2_fast(M - mn);
     l *= a;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] *= a;
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j) {
-      if (s0 + j >= ns) continue;
-      const float w = exp2_fast(ml[j][0] - mn);
-      l = __builtin_fmaf(w, ml[j][1], l);
+    for (int i = 0; i < BATCH; ++i) {
+      if (s0 + JOIN * i >= ns) continue;
+      const float w = exp2_fast(ml[i][0] - mn);
+      l = __builtin_fmaf(w, ml[i][1], l);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w, x[j][e], o[e]);
+      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w, x[i][e], o[e]);
     }
     M = mn;
   }
-  const float inv = 1.f / l;
-  u32x2 y = {pack2<E>(o[0] * inv, o[1] * inv), pack2<E>(o[2] * inv, o[3] * inv)};
-  if (l == 0.f) y = u32x2{0u, 0u};
-  *reinterpret_cast<u32x2*>(p.out + row * D + 4 * c) = y;
+  *reinterpret_cast<f32x4*>(&part[r][j][4 * c]) = o;
+  if (c == 0) *reinterpret_cast<f32x2*>(&part[r][j][D]) = f32x2{M, l};
+  __syncthreads();
+  if (j) return;
+  float top = kTreeNone, lt = 0.f;
+#pragma unroll
+  for (int i = 0; i < JOIN; ++i) top = fmaxf(top, part[r][i][D]);
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < JOIN; ++i) {
+    const float w = exp2_fast(part[r][i][D] - top);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(&part[r][i][4 * c]);
+    lt = __builtin_fmaf(w, part[r][i][D + 1], lt);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = __builtin_fmaf(w, x[e], y[e]);
+  }
+  const float inv = 1.f / lt;
+  u32x2 z = {pack2<E>(y[0] * inv, y[1] * inv), pack2<E>(y[2] * inv, y[3] * inv)};
+  if (lt == 0.f) z = u32x2{0u, 0u};
+  *reinterpret_cast<u32x2*>(p.out + row * D + 4 * c) = z;
 }
 
 // ===========================================================================
