@@ -258,17 +258,17 @@ int mt_topk_verify(const void* logits, const void* draft_logits, const int64_t* 
  * without entries counts nothing.  With T = temperature > 0,
  *   p = softmax(teacher / T) over the row's entries,
  *   *loss = T^2 / n sum_r sum_j p_j (log p_j - log softmax(logits / T)[index_j]),
- * n = *count = the rows with entries (0 of them: loss 0).  An index >= vocab makes
- * its row NaN.  fp32 arithmetic, the rows summed in 64 bits in a fixed order.
- * row_state [rows, 4] fp32, 16-byte aligned, is written for the backward:
+ * n = the rows with entries (0 of them: loss 0).  An index >= vocab makes its row
+ * NaN.  fp32 arithmetic, the rows summed in 64 bits in a fixed order.
+ * row_state [rows + 1, 4] fp32, 16-byte aligned, is written for the backward:
  *   dlogits = *grad T / n (softmax(logits / T) - P),  P[v] = sum of p_j with index_j = v,
  * contiguous [rows, vocab] in dtype, zero in rows without entries. */
 int mt_topk_distill_fwd(const void* logits, int64_t row_stride, const float* teacher, const int64_t* index,
                         int64_t rows, int vocab, int entries, float temperature, float* row_state, float* loss,
-                        float* count, int dtype, void* stream);
+                        int dtype, void* stream);
 int mt_topk_distill_bwd(const void* logits, int64_t row_stride, const float* teacher, const int64_t* index,
-                        const float* row_state, const float* count, const float* grad, void* dlogits, int64_t rows,
-                        int vocab, int entries, float temperature, int dtype, void* stream);
+                        const float* row_state, const float* grad, void* dlogits, int64_t rows, int vocab, int entries,
+                        float temperature, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -118,8 +118,8 @@ _OPS_SIGNATURES = {
     "mt_tree_commit": (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "mt_topk_verify_workspace_size": (_S, [_I, _I, _I, _I, _I]),
     "mt_topk_verify": (_I, [_P, _P, _P, _P, _P, _L, _P, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _P, _S, _P]),
-    "mt_topk_distill_fwd": (_I, [_P, _L, _P, _P, _L, _I, _I, _F, _P, _P, _P, _I, _P]),
-    "mt_topk_distill_bwd": (_I, [_P, _L, _P, _P, _P, _P, _P, _P, _L, _I, _I, _F, _I, _P]),
+    "mt_topk_distill_fwd": (_I, [_P, _L, _P, _P, _L, _I, _I, _F, _P, _P, _I, _P]),
+    "mt_topk_distill_bwd": (_I, [_P, _L, _P, _P, _P, _P, _P, _L, _I, _I, _F, _I, _P]),
 }
 
 

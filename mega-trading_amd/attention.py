@@ -314,21 +314,11 @@ def tree_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor, sin: to
     one per sequence, read when the kernel runs.  ``cos`` / ``sin`` are the
     RotaryEmbedding tables; positions past their last row take that row, so keep
     ``length`` plus the tree's depth within them."""
-    _check_nodes(query, key, key, (torch.float16, torch.bfloat16, torch.float32))
-    b, _, n, d = query.shape
-    if d % 8:
-        raise ValueError(f"tree_rope needs a head_dim that is a multiple of 8 (got {d})")
-    for name, tab in (("cos", cos), ("sin", sin)):
-        if tab.shape[-1] != d // 2 or not tab.is_floating_point():
-            raise ValueError(f"RoPE {name} table must be floating point with last dimension head_dim/2 = {d // 2}")
-        if tab.device != query.device:
-            raise RuntimeError(f"RoPE {name} table must be on the device of query")
-    rows = min(cos.numel(), sin.numel()) // (d // 2)
-    if rows < 1:
-        raise ValueError("the RoPE tables must have rows")
-    length_dev, length = _check_tree(parents, length, b, n, rows - 1, query.device)
+    _check_gpu(query)
     _native.ensure()
-    return _tree_rope(query, key, cos, sin, length_dev, length, parents)
+    if isinstance(length, torch.Tensor):
+        return _tree_rope(query, key, cos, sin, length, 0, parents)
+    return _tree_rope(query, key, cos, sin, None, length, parents)
 
 
 def tree_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
@@ -348,16 +338,16 @@ def tree_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, 
     A chain of one node is ``decode_attention`` with the new token's key and value
     outside the cache.  The caches are not written: ``tree_commit`` writes the
     nodes that the verification (``ops.topk_verify``) accepts."""
-    _check_nodes(query, key, value, tuple(_KERNEL_DTYPES))
-    b, hq, n, d = query.shape
-    if key.shape[1] * repeats != hq:
+    _check_gpu(query)
+    if query.ndim != 4 or key.ndim != 4:
+        raise ValueError("query, key and value must be [batch, heads, nodes, head_dim]")
+    if key.shape[1] * repeats != query.shape[1]:
         raise ValueError("query heads must equal key/value heads multiplied by repeats")
-    if d not in KERNEL_HEAD_DIMS:
-        raise ValueError(f"head_dim must be one of {KERNEL_HEAD_DIMS} (got {d})")
-    _check_caches((key_cache,), (value_cache,), key)
-    length_dev, length = _check_tree(parents, length, b, n, key_cache.shape[2], query.device)
+    scale = 1.0 / math.sqrt(max(query.shape[3], 1))
     _native.ensure()
-    return _tree_attn(query, key, value, key_cache, value_cache, length_dev, length, parents, 1.0 / math.sqrt(d))
+    if isinstance(length, torch.Tensor):
+        return _tree_attn(query, key, value, key_cache, value_cache, length, 0, parents, scale)
+    return _tree_attn(query, key, value, key_cache, value_cache, None, length, parents, scale)
 
 
 def tree_commit(keys, values, path: torch.Tensor, count: torch.Tensor, length, key_caches, value_caches) -> None:
@@ -372,7 +362,49 @@ def tree_commit(keys, values, path: torch.Tensor, count: torch.Tensor, length, k
     ``length`` as for ``tree_attention``: the cached tokens before this call, which
     are ``length + count`` after it.  Nodes outside the tree and positions at or
     past the capacity are skipped.  One launch for every 32 layers of one layout."""
-    keys, values, key_caches, value_caches = (list(x) for x in (keys, values, key_caches, value_caches))
+    keys, values, key_caches, value_caches = list(keys), list(values), list(key_caches), list(value_caches)
+    if not keys:
+        raise ValueError("keys, values, key_caches and value_caches must hold one tensor per layer, at least one")
+    _check_gpu(keys[0])
+    _native.ensure()
+    if isinstance(length, torch.Tensor):
+        _tree_commit(keys, values, path, count, length, 0, key_caches, value_caches)
+    else:
+        _tree_commit(keys, values, path, count, None, length, key_caches, value_caches)
+
+
+def _check_gpu(t: torch.Tensor) -> None:
+    if not t.is_cuda:
+        raise RuntimeError("hip attention backend requires ROCm GPU tensors")
+
+
+# The tree operators' checks for traced calls; libmt_torch.so makes them for the GPU's tensors
+def _check_tree_rope(query, key, cos, sin, length_dev, length, parents) -> None:
+    _check_nodes(query, key, key, (torch.float16, torch.bfloat16, torch.float32))
+    b, _, n, d = query.shape
+    if d % 8 or not d:
+        raise ValueError(f"tree_rope needs a head_dim that is a multiple of 8 (got {d})")
+    for name, tab in (("cos", cos), ("sin", sin)):
+        if not tab.ndim or tab.shape[-1] != d // 2 or not tab.is_floating_point():
+            raise ValueError(f"RoPE {name} table must be floating point with last dimension head_dim/2 = {d // 2}")
+        if tab.device != query.device:
+            raise RuntimeError("RoPE tables must be on the device of query")
+    rows = min(cos.numel(), sin.numel()) // (d // 2)
+    if rows < 1:
+        raise ValueError("the RoPE tables must have rows")
+    _check_tree(parents, length_dev, length, b, n, rows - 1, query.device)
+
+
+def _check_tree_attention(query, key, value, key_cache, value_cache, length_dev, length, parents) -> None:
+    _check_nodes(query, key, value, tuple(_KERNEL_DTYPES))
+    b, _, n, d = query.shape
+    if d not in KERNEL_HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {KERNEL_HEAD_DIMS} (got {d})")
+    _check_caches(key_cache, value_cache, key)
+    _check_tree(parents, length_dev, length, b, n, key_cache.shape[2], query.device)
+
+
+def _check_tree_commit(keys, values, path, count, length_dev, length, key_caches, value_caches) -> None:
     if not keys or not len(keys) == len(values) == len(key_caches) == len(value_caches):
         raise ValueError("keys, values, key_caches and value_caches must hold one tensor per layer, at least one")
     first = keys[0]
@@ -382,26 +414,22 @@ def tree_commit(keys, values, path: torch.Tensor, count: torch.Tensor, length, k
             raise ValueError("keys and values must share one shape [batch, heads, nodes, head_dim]")
         if t.dtype != first.dtype or t.device != first.device:
             raise RuntimeError("keys and values must share one dtype and device")
-    _check_caches(key_caches, value_caches, first)
-    for t in (*key_caches, *value_caches):
-        if t.shape != key_caches[0].shape:
+    for kc, vc in zip(key_caches, value_caches):
+        _check_caches(kc, vc, first)
+        if kc.shape != key_caches[0].shape:
             raise ValueError("the caches must share one shape")
-        if t.stride(-1) != 1:
+        if kc.stride(-1) != 1 or vc.stride(-1) != 1:
             raise ValueError("the caches must have a unit last-dim stride")
     b, _, n, _ = first.shape
     for name, t, shape in (("path", path, (b, n)), ("count", count, (b,))):
         if t.dtype != torch.int32 or tuple(t.shape) != shape:
             raise ValueError(f"{name} must be int32 of shape {list(shape)} (got {t.dtype}, {list(t.shape)})")
         if t.device != first.device:
-            raise RuntimeError(f"{name} must be on the device of the keys")
-    length_dev, length = _check_length(length, b, key_caches[0].shape[2], first.device)
-    _native.ensure()
-    _tree_commit(keys, values, path, count, length_dev, length, key_caches, value_caches)
+            raise RuntimeError(f"{name} must be on the device of the other arguments")
+    _check_length(length_dev, length, b, key_caches[0].shape[2], first.device)
 
 
 def _check_nodes(query, key, value, dtypes) -> None:
-    if query.device.type != "cuda":
-        raise RuntimeError("hip attention backend requires ROCm GPU tensors")
     if query.dtype not in dtypes:
         raise RuntimeError("unsupported dtype %s (%s)" % (query.dtype, ", ".join(str(t) for t in dtypes)))
     if query.ndim != 4 or key.ndim != 4 or value.ndim != 4:
@@ -419,34 +447,31 @@ def _check_nodes(query, key, value, dtypes) -> None:
             raise RuntimeError("query, key and value must share one dtype and device")
 
 
-def _check_caches(key_caches, value_caches, key) -> None:
-    for kc, vc in zip(key_caches, value_caches):
-        if kc.ndim != 4 or kc.shape != vc.shape:
-            raise ValueError("key and value caches must have the same shape [batch, heads, capacity, head_dim]")
-        if kc.shape[:2] != key.shape[:2] or kc.shape[3] != key.shape[3]:
-            raise ValueError("the caches must have the batch, heads and head_dim of the nodes' keys")
-        for t in (kc, vc):
-            if t.dtype != key.dtype or t.device != key.device:
-                raise RuntimeError("the caches must have the dtype and device of the nodes' keys")
+def _check_caches(key_cache, value_cache, key) -> None:
+    if key_cache.ndim != 4 or key_cache.shape != value_cache.shape:
+        raise ValueError("key and value caches must have the same shape [batch, heads, capacity, head_dim]")
+    if key_cache.shape[:2] != key.shape[:2] or key_cache.shape[3] != key.shape[3]:
+        raise ValueError("the caches must have the batch, heads and head_dim of the nodes' keys")
+    for t in (key_cache, value_cache):
+        if t.dtype != key.dtype or t.device != key.device:
+            raise RuntimeError("the caches must have the dtype and device of the nodes' keys")
 
 
-def _check_length(length, b: int, most: int, device):
-    """(device length or None, int length): the cached tokens of every sequence."""
-    if isinstance(length, torch.Tensor):
-        if length.dtype != torch.int32 or length.ndim > 1 or length.numel() not in (1, b) or length.device != device:
+def _check_length(length_dev, length, b: int, most: int, device) -> None:
+    if length_dev is not None:
+        if (length_dev.dtype != torch.int32 or length_dev.ndim > 1 or length_dev.numel() not in (1, b)
+                or length_dev.device != device):
             raise ValueError("a tensor length must be int32 of one element or one per sequence, on the nodes' device")
-        return length, 0
-    if not 0 <= length <= most:
+    elif not 0 <= length <= most:
         raise ValueError(f"length {length} outside [0, {most}]")
-    return None, int(length)
 
 
-def _check_tree(parents, length, b: int, n: int, most: int, device):
+def _check_tree(parents, length_dev, length, b: int, n: int, most: int, device) -> None:
     if parents.dtype != torch.int32 or tuple(parents.shape) not in ((n,), (b, n)):
         raise ValueError(f"parents must be int32 of shape [{n}] or [{b}, {n}] (got {parents.dtype}, {list(parents.shape)})")
     if parents.device != device:
-        raise RuntimeError("parents must be on the device of query")
-    return _check_length(length, b, most, device)
+        raise RuntimeError("parents must be on the device of the other arguments")
+    _check_length(length_dev, length, b, most, device)
 
 
 # ---------------------------------------------------------------------------
@@ -630,17 +655,19 @@ _LIB.define("tree_commit(Tensor[] keys, Tensor[] values, Tensor path, Tensor cou
 
 @torch.library.register_fake("mega_trading_amd::tree_rope")
 def _tree_rope_fake(q, k, cos, sin, length_dev, length, parents):
+    _check_tree_rope(q, k, cos, sin, length_dev, length, parents)
     return q.new_empty(q.shape), k.new_empty(k.shape)
 
 
 @torch.library.register_fake("mega_trading_amd::tree_attn")
 def _tree_attn_fake(q, k, v, k_cache, v_cache, length_dev, length, parents, scale):
+    _check_tree_attention(q, k, v, k_cache, v_cache, length_dev, length, parents)
     return q.new_empty(q.shape)
 
 
 @torch.library.register_fake("mega_trading_amd::tree_commit")
 def _tree_commit_fake(keys, values, path, count, length_dev, length, key_caches, value_caches):
-    return None
+    _check_tree_commit(keys, values, path, count, length_dev, length, key_caches, value_caches)
 
 
 # the ops as the functions above call them

@@ -29,13 +29,13 @@ struct DistillParams {
   int V, K;
   int64_t rows;
   float inv_t;
-  // [rows, 4]: the row's sum of p (log p - log q), the largest logit M, the sum of exp((x - M) / T)
-  // (two numbers where one, the logarithm, would lose bits with the logits' size), 1 (0 without entries)
+  // [rows + 1, 4]: the row's sum of p (log p - log q), the largest logit M, the sum of exp((x - M) / T)
+  // (two numbers where one, the logarithm, would lose bits with the logits' size), 1 (0 without entries);
+  // then n
   float* row;
   // backward
-  const float* count;  // n
-  const float* grad;   // incoming gradient
-  void* dx;            // [rows, V] contiguous
+  const float* grad;  // incoming gradient
+  void* dx;           // [rows, V] contiguous
 };
 
 template <bool MAX>
@@ -150,8 +150,7 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams a) {
 }
 
 // loss = T^2 sum / n and n, in a fixed order and 64 bits: one workgroup.
-__global__ __launch_bounds__(1024) void distill_sum_kernel(const float* row, int64_t rows, float t2, float* loss,
-                                                           float* count) {
+__global__ __launch_bounds__(1024) void distill_sum_kernel(float* row, int64_t rows, float t2, float* loss) {
   __shared__ double part[2][16];
   double s = 0., n = 0.;
   for (int64_t i = threadIdx.x; i < rows; i += 8 * 1024) {
@@ -181,7 +180,7 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* row, int
       n += part[1][w];
     }
     *loss = n > 0. ? (float)(s * t2 / n) : 0.f;
-    *count = (float)n;
+    row[4 * rows] = (float)n;
   }
 }
 
@@ -211,7 +210,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
     bad |= e.p[j] != 0.f && e.idx[j] >= a.V;
   }
   const float c2 = a.inv_t * kLog2e, M = r[1], inv = 1.f / r[2];
-  float scale = *a.grad / (*a.count * a.inv_t);
+  float scale = *a.grad / (a.row[4 * a.rows] * a.inv_t);
   if (__syncthreads_or(bad)) scale = __builtin_nanf("");
   const float qs = inv * scale;
   for (int c0 = tid; c0 < nvec; c0 += 256 * kDistillAhead) {

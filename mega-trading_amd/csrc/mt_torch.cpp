@@ -309,12 +309,79 @@ Tree tree(const std::optional<at::Tensor>& parents, const std::optional<at::Tens
   return t;
 }
 
+// The checks of the calls, here for the GPU's tensors and in Python (attention.py, ops.py) for traced ones: in
+// Python they cost as much as the rest of a small call (5 nodes on a cache 11.4 -> 7.2 us a call, the write
+// into 8 layers' caches 35.2 -> 10.5).
+void check_nodes(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, bool fp32) {
+  const at::ScalarType t = q.scalar_type();
+  TORCH_CHECK(t == at::kBFloat16 || t == at::kHalf || (fp32 && t == at::kFloat), "unsupported dtype ", t);
+  TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && v.dim() == 4,
+                    "query, key and value must be [batch, heads, nodes, head_dim]");
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes(), "key and value must have the same shape");
+  TORCH_CHECK_VALUE(k.size(0) == q.size(0) && k.size(2) == q.size(2) && k.size(3) == q.size(3),
+                    "query, key and value must agree on batch, nodes and head_dim");
+  TORCH_CHECK_VALUE(k.size(1) > 0 && q.size(1) > 0 && q.size(1) % k.size(1) == 0,
+                    "query heads must be a positive multiple of the key/value heads");
+  TORCH_CHECK_VALUE(q.size(0) > 0 && q.size(2) >= 1 && q.size(2) <= 64, "need a batch and 1 to 64 nodes (got ", q.size(0),
+                    ", ", q.size(2), ")");
+  for (const at::Tensor* x : {&k, &v})
+    TORCH_CHECK(x->scalar_type() == t && x->device() == q.device(), "query, key and value must share one dtype and device");
+}
+void check_caches(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& key) {
+  TORCH_CHECK_VALUE(kc.dim() == 4 && kc.sizes() == vc.sizes(),
+                    "key and value caches must have the same shape [batch, heads, capacity, head_dim]");
+  TORCH_CHECK_VALUE(kc.size(0) == key.size(0) && kc.size(1) == key.size(1) && kc.size(3) == key.size(3),
+                    "the caches must have the batch, heads and head_dim of the nodes' keys");
+  for (const at::Tensor* x : {&kc, &vc})
+    TORCH_CHECK(x->scalar_type() == key.scalar_type() && x->device() == key.device(),
+                "the caches must have the dtype and device of the nodes' keys");
+}
+void check_length(const std::optional<at::Tensor>& length_dev, int64_t length, int64_t b, int64_t most, at::Device device) {
+  if (length_dev.has_value() && length_dev->defined()) {
+    TORCH_CHECK_VALUE(length_dev->scalar_type() == at::kInt && length_dev->dim() <= 1 &&
+                          (length_dev->numel() == 1 || length_dev->numel() == b) && length_dev->device() == device,
+                      "a tensor length must be int32 of one element or one per sequence, on the nodes' device");
+  } else {
+    TORCH_CHECK_VALUE(length >= 0 && length <= most, "length ", length, " outside [0, ", most, "]");
+  }
+}
+void check_ints(const char* name, const at::Tensor& t, at::ScalarType type, at::IntArrayRef shape, at::Device device) {
+  TORCH_CHECK_VALUE(t.scalar_type() == type && t.sizes() == shape, name, " must be ",
+                    type == at::kInt ? "int32" : type == at::kLong ? "int64" : "float32", " of shape ", shape, " (got ",
+                    t.scalar_type(), ", ", t.sizes(), ")");
+  TORCH_CHECK(t.device() == device, name, " must be on the device of the other arguments");
+}
+void check_float(const char* name, const at::Tensor& t) {
+  const at::ScalarType x = t.scalar_type();
+  TORCH_CHECK(x == at::kBFloat16 || x == at::kHalf || x == at::kFloat, name, " dtype ", x,
+              " unsupported (bfloat16, float16 or float32)");
+}
+void check_parents(const at::Tensor& t, int64_t b, int64_t n, at::Device device) {
+  if (t.dim() == 1) {
+    check_ints("parents", t, at::kInt, {n}, device);
+  } else {
+    check_ints("parents", t, at::kInt, {b, n}, device);
+  }
+}
+
 // in place where the kernels can read it, else a copy
 at::Tensor rows16(const at::Tensor& t) { return kernel_ready(t) ? t : flat(t); }
 
 std::tuple<at::Tensor, at::Tensor> tree_rope(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& cos,
                                              const at::Tensor& sin, const std::optional<at::Tensor>& length_dev,
                                              int64_t length, const at::Tensor& parents) {
+  check_nodes(q_in, k_in, k_in, true);
+  const int64_t half = q_in.size(3) / 2;
+  TORCH_CHECK_VALUE(half && q_in.size(3) % 8 == 0, "tree_rope needs a head_dim that is a multiple of 8 (got ", q_in.size(3), ")");
+  for (const at::Tensor* t : {&cos, &sin}) {
+    TORCH_CHECK_VALUE(t->dim() > 0 && t->size(-1) == half && t->is_floating_point(),
+                      "RoPE cos / sin table must be floating point with last dimension head_dim/2 = ", half);
+    TORCH_CHECK(t->device() == q_in.device(), "RoPE tables must be on the device of query");
+  }
+  const int64_t rows = std::min(cos.numel(), sin.numel()) / half;
+  TORCH_CHECK_VALUE(rows > 0, "the RoPE tables must have rows");
+  check_parents(parents, q_in.size(0), q_in.size(2), q_in.device());
+  check_length(length_dev, length, q_in.size(0), rows - 1, q_in.device());
   const c10::DeviceGuard guard(q_in.device());
   const at::Tensor q = rows16(q_in), k = rows16(k_in);
   const int64_t b = q.size(0), hq = q.size(1), n = q.size(2), d = q.size(3), hkv = k.size(1);
@@ -326,7 +393,7 @@ std::tuple<at::Tensor, at::Tensor> tree_rope(const at::Tensor& q_in, const at::T
   put_strides(s.data() + 4, k);
   s[3] = s[7] = 1;
   check_rc(mt_tree_rope(q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), s.data(), f32_ptr(cs), f32_ptr(sn),
-                        int(std::min(cs.numel(), sn.numel()) / (d / 2)), t.parent(), t.parents_stride, t.length_dev(),
+                        int(rows), t.parent(), t.parents_stride, t.length_dev(),
                         t.length_stride, int(length), int(b), int(hq), int(hkv), int(n), int(d), dtype_code(q),
                         stream_of(q)),
            "mt_tree_rope");
@@ -336,6 +403,12 @@ std::tuple<at::Tensor, at::Tensor> tree_rope(const at::Tensor& q_in, const at::T
 at::Tensor tree_attn(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in, const at::Tensor& kc_in,
                      const at::Tensor& vc_in, const std::optional<at::Tensor>& length_dev, int64_t length,
                      const at::Tensor& parents, double scale) {
+  check_nodes(q_in, k_in, v_in, false);
+  const int64_t hd = q_in.size(3);
+  TORCH_CHECK_VALUE(hd == 32 || hd == 64 || hd == 128, "head_dim must be one of (32, 64, 128) (got ", hd, ")");
+  check_caches(kc_in, vc_in, k_in);
+  check_parents(parents, q_in.size(0), q_in.size(2), q_in.device());
+  check_length(length_dev, length, q_in.size(0), kc_in.size(2), q_in.device());
   const c10::DeviceGuard guard(q_in.device());
   const at::Tensor q = rows16(q_in), k = rows16(k_in), v = rows16(v_in), kc = rows16(kc_in), vc = rows16(vc_in);
   const int64_t b = q.size(0), hq = q.size(1), n = q.size(2), d = q.size(3), hkv = k.size(1), cap = kc.size(2);
@@ -361,9 +434,24 @@ at::Tensor tree_attn(const at::Tensor& q_in, const at::Tensor& k_in, const at::T
 void tree_commit(at::TensorList keys, at::TensorList values, const at::Tensor& path_in, const at::Tensor& count_in,
                  const std::optional<at::Tensor>& length_dev, int64_t length, at::TensorList key_caches,
                  at::TensorList value_caches) {
-  TORCH_CHECK(!keys.empty() && keys.size() == values.size() && keys.size() == key_caches.size() &&
-                  keys.size() == value_caches.size(),
-              "keys, values and the caches must hold one tensor per layer");
+  TORCH_CHECK_VALUE(!keys.empty() && keys.size() == values.size() && keys.size() == key_caches.size() &&
+                        keys.size() == value_caches.size(),
+                    "keys, values, key_caches and value_caches must hold one tensor per layer, at least one");
+  check_nodes(keys[0], keys[0], keys[0], false);
+  for (size_t l = 0; l < keys.size(); ++l) {
+    for (const at::Tensor* x : {&keys[l], &values[l]}) {
+      TORCH_CHECK_VALUE(x->sizes() == keys[0].sizes(), "keys and values must share one shape [batch, heads, nodes, head_dim]");
+      TORCH_CHECK(x->scalar_type() == keys[0].scalar_type() && x->device() == keys[0].device(),
+                  "keys and values must share one dtype and device");
+    }
+    check_caches(key_caches[l], value_caches[l], keys[0]);
+    TORCH_CHECK_VALUE(key_caches[l].sizes() == key_caches[0].sizes(), "the caches must share one shape");
+    TORCH_CHECK_VALUE(key_caches[l].stride(3) == 1 && value_caches[l].stride(3) == 1,
+                      "the caches must have a unit last-dim stride");
+  }
+  check_ints("path", path_in, at::kInt, {keys[0].size(0), keys[0].size(2)}, keys[0].device());
+  check_ints("count", count_in, at::kInt, {keys[0].size(0)}, keys[0].device());
+  check_length(length_dev, length, keys[0].size(0), key_caches[0].size(2), keys[0].device());
   const c10::DeviceGuard guard(keys[0].device());
   const at::Tensor path = path_in.contiguous(), count = count_in.contiguous();
   const Tree t = tree(std::nullopt, length_dev);
@@ -407,6 +495,23 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> topk_verify(const at::Tensor& log
                                                            const at::Tensor& tokens_in, const at::Tensor& parents,
                                                            const at::Tensor& uniform_in, const at::Tensor& noise,
                                                            int64_t k) {
+  TORCH_CHECK_VALUE(logits.dim() == 3, "logits must have shape [batch, nodes, vocab]");
+  check_float("logits", logits);
+  {
+    const int64_t b = logits.size(0), n = logits.size(1), v = logits.size(2);
+    const at::Device dev = logits.device();
+    TORCH_CHECK_VALUE(n >= 1 && n <= 64, "need 1 to 64 nodes (got ", n, ")");
+    TORCH_CHECK_VALUE(1 <= k && k <= v && v <= 32768, "need 1 <= k <= vocab <= 32768 (k=", k, ", vocab=", v, ")");
+    check_ints("tokens", tokens_in, at::kLong, {b, n}, dev);
+    check_parents(parents, b, n, dev);
+    check_ints("uniform", uniform_in, at::kFloat, {b, n}, dev);
+    check_ints("noise", noise, at::kFloat, {b, v}, dev);
+    if (draft.has_value() && draft->defined()) {
+      TORCH_CHECK_VALUE(draft->sizes() == logits.sizes(), "draft_logits must have the shape of logits");
+      TORCH_CHECK(draft->scalar_type() == logits.scalar_type() && draft->device() == dev,
+                  "draft_logits must have the dtype and device of logits");
+    }
+  }
   const c10::DeviceGuard guard(logits.device());
   auto unit = [](const at::Tensor& x) { return x.stride(-1) == 1 ? x : x.contiguous(); };
   const bool drafted = draft.has_value() && draft->defined();
@@ -436,28 +541,41 @@ at::Tensor plain_rows(const at::Tensor& x) {
 }
 int64_t row_stride(const at::Tensor& r) { return r.size(0) > 1 ? r.stride(0) : r.size(1); }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> topk_distill_fwd(const at::Tensor& logits, const at::Tensor& teacher,
-                                                                const at::Tensor& index, double temperature) {
+void check_distill(const at::Tensor& x, const at::Tensor& y, const at::Tensor& i) {
+  check_float("logits", x);
+  check_float("teacher_logits", y);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "logits must have shape [..., vocab]");
+  TORCH_CHECK_VALUE(y.dim() == x.dim() && y.sizes().slice(0, y.dim() - 1) == x.sizes().slice(0, x.dim() - 1),
+                    "teacher_logits must have shape [..., entries] with the rows of logits");
+  TORCH_CHECK_VALUE(i.sizes() == y.sizes(), "teacher_indices must have the shape of teacher_logits");
+  TORCH_CHECK_VALUE(i.scalar_type() == at::kLong || i.scalar_type() == at::kInt,
+                    "teacher_indices must be an integer tensor (int32 or int64)");
+  TORCH_CHECK_VALUE(y.size(-1) >= 1 && y.size(-1) <= 1024, "need 1 to 1024 teacher logits a row (got ", y.size(-1), ")");
+  TORCH_CHECK(y.device() == x.device() && i.device() == x.device(), "the teacher's tensors must be on the device of logits");
+}
+
+std::tuple<at::Tensor, at::Tensor> topk_distill_fwd(const at::Tensor& logits, const at::Tensor& teacher,
+                                                    const at::Tensor& index, double temperature) {
+  check_distill(logits, teacher, index);
   const c10::DeviceGuard guard(logits.device());
   const at::Tensor x = plain_rows(logits), y = teacher.to(at::kFloat).contiguous(), i = index.to(at::kLong).contiguous();
   const auto f32 = x.options().dtype(at::kFloat);
-  const at::Tensor loss = at::empty({}, f32), state = at::empty({x.size(0), 4}, f32), count = at::empty({}, f32);
+  const at::Tensor loss = at::empty({}, f32), state = at::empty({x.size(0) + 1, 4}, f32);
   check_rc(mt_topk_distill_fwd(x.data_ptr(), row_stride(x), f32_ptr(y), static_cast<const int64_t*>(i.data_ptr()),
                                x.size(0), int(x.size(1)), int(y.size(-1)), float(temperature), f32_ptr(state),
-                               f32_ptr(loss), f32_ptr(count), dtype_code(x), stream_of(x)),
+                               f32_ptr(loss), dtype_code(x), stream_of(x)),
            "mt_topk_distill_fwd");
-  return {loss, state, count};
+  return {loss, state};
 }
 
 at::Tensor topk_distill_bwd(const at::Tensor& logits, const at::Tensor& teacher, const at::Tensor& index,
-                            const at::Tensor& state, const at::Tensor& count, const at::Tensor& grad,
-                            double temperature) {
+                            const at::Tensor& state, const at::Tensor& grad, double temperature) {
   const c10::DeviceGuard guard(logits.device());
   const at::Tensor x = plain_rows(logits), y = teacher.to(at::kFloat).contiguous(), i = index.to(at::kLong).contiguous();
   const at::Tensor g = grad.to(at::kFloat).contiguous(), dx = at::empty(logits.sizes(), logits.options());
   check_rc(mt_topk_distill_bwd(x.data_ptr(), row_stride(x), f32_ptr(y), static_cast<const int64_t*>(i.data_ptr()),
-                               f32_ptr(state), f32_ptr(count), f32_ptr(g), dx.data_ptr(), x.size(0), int(x.size(1)),
-                               int(y.size(-1)), float(temperature), dtype_code(x), stream_of(x)),
+                               f32_ptr(state), f32_ptr(g), dx.data_ptr(), x.size(0), int(x.size(1)), int(y.size(-1)),
+                               float(temperature), dtype_code(x), stream_of(x)),
            "mt_topk_distill_bwd");
   return dx;
 }
@@ -980,19 +1098,19 @@ struct DistillFn : torch::autograd::Function<DistillFn> {
                                const at::Tensor& index, double temperature) {
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = MT_OP(topk_distill_fwd);
-    auto [loss, state, count] = op.call(logits, teacher, index, temperature);
-    ctx->save_for_backward({logits, teacher, index, state, count});
+    auto [loss, state] = op.call(logits, teacher, index, temperature);
+    ctx->save_for_backward({logits, teacher, index, state});
     ctx->saved_data["temperature"] = temperature;
-    ctx->mark_non_differentiable({state, count});
+    ctx->mark_non_differentiable({state});
     ctx->set_materialize_grads(false);
-    return {loss, state, count};
+    return {loss, state};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     if (!g[0].defined() || !ctx->needs_input_grad(0)) return variable_list(4);
     const auto s = ctx->get_saved_variables();
     static const auto op = MT_OP(topk_distill_bwd);
     variable_list r(4);
-    r[0] = op.call(s[0], s[1], s[2], s[3], s[4], g[0], ctx->saved_data["temperature"].toDouble());
+    r[0] = op.call(s[0], s[1], s[2], s[3], g[0], ctx->saved_data["temperature"].toDouble());
     return r;
   }
 };
@@ -1084,11 +1202,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> fused_linear_ce_ad(const at::Tens
   return {r[0], r[1], r[2]};
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> topk_distill_fwd_ad(const at::Tensor& logits, const at::Tensor& teacher,
-                                                                   const at::Tensor& index, double temperature) {
+std::tuple<at::Tensor, at::Tensor> topk_distill_fwd_ad(const at::Tensor& logits, const at::Tensor& teacher,
+                                                       const at::Tensor& index, double temperature) {
   if (!records(logits, teacher)) MT_BELOW(topk_distill_fwd, logits, teacher, index, temperature);
   auto r = DistillFn::apply(logits, teacher, index, temperature);
-  return {r[0], r[1], r[2]};
+  return {r[0], r[1]};
 }
 
 // The write into the caches has no result that could carry a refusal: it refuses at once.

@@ -423,14 +423,14 @@ int mt_topk_verify(const void* logits, const void* draft_logits, const int64_t* 
 
 int mt_topk_distill_fwd(const void* logits, int64_t row_stride, const float* teacher, const int64_t* index,
                         int64_t rows, int vocab, int entries, float temperature, float* row_state, float* loss,
-                        float* count, int dtype, void* stream) {
+                        int dtype, void* stream) {
   int rc;
   if ((rc = check_distill(row_stride, rows, vocab, entries, temperature, dtype))) return rc;
-  if (!loss || !count) return fail(MT_E_NULL, "loss and count must be non-NULL");
+  if (!loss || !row_state) return fail(MT_E_NULL, "loss and row_state must be non-NULL");
+  if (!aligned16(row_state)) return fail(MT_E_STRIDE, "row_state must be 16-byte aligned");
   if (rows > 0) {
     if ((rc = check_type_aligned("logits", logits, dtype))) return rc;
-    if (!teacher || !index || !row_state) return fail(MT_E_NULL, "teacher, index and row_state must be non-NULL");
-    if (!aligned16(row_state)) return fail(MT_E_STRIDE, "row_state must be 16-byte aligned");
+    if (!teacher || !index) return fail(MT_E_NULL, "teacher and index must be non-NULL");
   }
   mt::DistillParams p{};
   p.x = logits;
@@ -451,20 +451,20 @@ int mt_topk_distill_fwd(const void* logits, int64_t row_stride, const float* tea
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail((int)e, "distillation launch failed: %s", hipGetErrorString(e));
   }
-  hipLaunchKernelGGL(mt::distill_sum_kernel, dim3(1), dim3(1024), 0, st, row_state, rows, temperature * temperature, loss,
-                     count);
+  hipLaunchKernelGGL(mt::distill_sum_kernel, dim3(1), dim3(1024), 0, st, row_state, rows, temperature * temperature,
+                     loss);
   return launched("distillation");
 }
 
 int mt_topk_distill_bwd(const void* logits, int64_t row_stride, const float* teacher, const int64_t* index,
-                        const float* row_state, const float* count, const float* grad, void* dlogits, int64_t rows,
-                        int vocab, int entries, float temperature, int dtype, void* stream) {
+                        const float* row_state, const float* grad, void* dlogits, int64_t rows, int vocab, int entries,
+                        float temperature, int dtype, void* stream) {
   int rc;
   if ((rc = check_distill(row_stride, rows, vocab, entries, temperature, dtype))) return rc;
   if (rows == 0) return ok();
   if ((rc = check_type_aligned("logits", logits, dtype)) || (rc = check_type_aligned("dlogits", dlogits, dtype))) return rc;
-  if (!teacher || !index || !row_state || !count || !grad)
-    return fail(MT_E_NULL, "teacher, index, row_state, count and grad must be non-NULL");
+  if (!teacher || !index || !row_state || !grad)
+    return fail(MT_E_NULL, "teacher, index, row_state and grad must be non-NULL");
   if (!aligned16(row_state)) return fail(MT_E_STRIDE, "row_state must be 16-byte aligned");
   mt::DistillParams p{};
   p.x = logits;
@@ -476,7 +476,6 @@ int mt_topk_distill_bwd(const void* logits, int64_t row_stride, const float* tea
   p.rows = rows;
   p.inv_t = 1.f / temperature;
   p.row = const_cast<float*>(row_state);
-  p.count = count;
   p.grad = grad;
   p.dx = dlogits;
   const dim3 grid((unsigned)rows);

@@ -198,6 +198,57 @@ def _check_device_dtype(t: torch.Tensor, name: str) -> None:
         raise RuntimeError(f"{name} dtype {t.dtype} unsupported (bfloat16, float16 or float32)")
 
 
+def _check_gpu(t: torch.Tensor, name: str) -> None:
+    if not t.is_cuda or not torch.version.hip:
+        raise RuntimeError(f"{name} must be on a ROCm GPU (got device {t.device})")
+
+
+def _check_dtype(t: torch.Tensor, name: str) -> None:
+    if t.dtype not in _DT:
+        raise RuntimeError(f"{name} dtype {t.dtype} unsupported (bfloat16, float16 or float32)")
+
+
+# The checks of topk_verify and topk_distillation for traced calls; libmt_torch.so makes them for the GPU's
+def _check_verify(logits, draft_logits, tokens, parents, uniform, noise, k) -> None:
+    _check_dtype(logits, "logits")
+    if logits.ndim != 3:
+        raise ValueError("logits must have shape [batch, nodes, vocab]")
+    b, n, vocab = logits.shape
+    if not 1 <= n <= MAX_TREE_NODES:
+        raise ValueError(f"need 1 to {MAX_TREE_NODES} nodes (got {n})")
+    if not 1 <= k <= vocab or vocab > MAX_SAMPLE_VOCAB:
+        raise ValueError(f"need 1 <= k <= vocab <= {MAX_SAMPLE_VOCAB} (k={k}, vocab={vocab})")
+    for name, t, dtype, shapes in (("tokens", tokens, torch.int64, ((b, n),)), ("parents", parents, torch.int32, ((n,), (b, n))),
+                                   ("uniform", uniform, torch.float32, ((b, n),)),
+                                   ("noise", noise, torch.float32, ((b, vocab),))):
+        if t.dtype != dtype or tuple(t.shape) not in shapes:
+            raise ValueError(f"{name} must be {dtype} of shape {list(shapes[-1])} (got {t.dtype}, {list(t.shape)})")
+        if t.device != logits.device:
+            raise RuntimeError(f"{name} must be on the device of logits")
+    if draft_logits is not None:
+        if draft_logits.shape != logits.shape:
+            raise ValueError("draft_logits must have the shape of logits")
+        if draft_logits.dtype != logits.dtype or draft_logits.device != logits.device:
+            raise RuntimeError("draft_logits must have the dtype and device of logits")
+
+
+def _check_distillation(logits, teacher_logits, teacher_indices) -> None:
+    _check_dtype(logits, "logits")
+    _check_dtype(teacher_logits, "teacher_logits")
+    if logits.ndim < 1 or logits.shape[-1] < 1:
+        raise ValueError("logits must have shape [..., vocab]")
+    if teacher_logits.shape[:-1] != logits.shape[:-1] or teacher_logits.ndim != logits.ndim:
+        raise ValueError("teacher_logits must have shape [..., entries] with the rows of logits")
+    if teacher_indices.shape != teacher_logits.shape:
+        raise ValueError("teacher_indices must have the shape of teacher_logits")
+    if teacher_indices.dtype not in (torch.int32, torch.int64):
+        raise ValueError("teacher_indices must be an integer tensor (int32 or int64)")
+    if not 1 <= teacher_logits.shape[-1] <= MAX_TEACHER_ENTRIES:
+        raise ValueError(f"need 1 to {MAX_TEACHER_ENTRIES} teacher logits a row (got {teacher_logits.shape[-1]})")
+    if teacher_logits.device != logits.device or teacher_indices.device != logits.device:
+        raise RuntimeError("the teacher's tensors must be on the device of logits")
+
+
 def _check_norm(hidden: torch.Tensor, weight: torch.Tensor) -> None:
     _check_device_dtype(hidden, "hidden")
     d = hidden.shape[-1] if hidden.ndim else 0
@@ -279,26 +330,7 @@ def topk_verify(
     them), ``count`` [B] int32 their number, ``token`` [B, 1] int64 the drawn token.
     A sequence whose node 0 is padding has count 0 and token 0.  NaN and -inf logits
     count as the lowest fp32 value, +inf as the highest."""
-    _check_device_dtype(logits, "logits")
-    if logits.ndim != 3:
-        raise ValueError("logits must have shape [batch, nodes, vocab]")
-    b, n, vocab = logits.shape
-    if not 1 <= n <= MAX_TREE_NODES:
-        raise ValueError(f"need 1 to {MAX_TREE_NODES} nodes (got {n})")
-    if not 1 <= k <= vocab or vocab > MAX_SAMPLE_VOCAB:
-        raise ValueError(f"need 1 <= k <= vocab <= {MAX_SAMPLE_VOCAB} (k={k}, vocab={vocab})")
-    for name, t, dtype, shapes in (("tokens", tokens, torch.int64, ((b, n),)), ("parents", parents, torch.int32, ((n,), (b, n))),
-                                   ("uniform", uniform, torch.float32, ((b, n),)),
-                                   ("noise", noise, torch.float32, ((b, vocab),))):
-        if t.dtype != dtype or tuple(t.shape) not in shapes:
-            raise ValueError(f"{name} must be {dtype} of shape {list(shapes[-1])} (got {t.dtype}, {list(t.shape)})")
-        if t.device != logits.device:
-            raise RuntimeError(f"{name} must be on the device of logits")
-    if draft_logits is not None:
-        if draft_logits.shape != logits.shape:
-            raise ValueError("draft_logits must have the shape of logits")
-        if draft_logits.dtype != logits.dtype or draft_logits.device != logits.device:
-            raise RuntimeError("draft_logits must have the dtype and device of logits")
+    _check_gpu(logits, "logits")
     _native.ensure()
     return _topk_verify(logits, draft_logits, tokens, parents, uniform, noise, k)
 
@@ -321,24 +353,11 @@ def topk_distillation(
     ``logits`` and ``teacher_logits`` are bf16, fp16 or fp32, any vocabulary size;
     arithmetic and the scalar loss are fp32.  The gradient is the student's alone,
     rounded once to its dtype; the teacher gets none."""
-    _check_device_dtype(logits, "logits")
-    _check_device_dtype(teacher_logits, "teacher_logits")
-    if logits.ndim < 1 or logits.shape[-1] < 1:
-        raise ValueError("logits must have shape [..., vocab]")
-    if teacher_logits.shape[:-1] != logits.shape[:-1] or teacher_logits.ndim != logits.ndim:
-        raise ValueError("teacher_logits must have shape [..., entries] with the rows of logits")
-    if teacher_indices.shape != teacher_logits.shape:
-        raise ValueError("teacher_indices must have the shape of teacher_logits")
-    if teacher_indices.dtype not in (torch.int32, torch.int64):
-        raise ValueError("teacher_indices must be an integer tensor (int32 or int64)")
-    if not 1 <= teacher_logits.shape[-1] <= MAX_TEACHER_ENTRIES:
-        raise ValueError(f"need 1 to {MAX_TEACHER_ENTRIES} teacher logits a row (got {teacher_logits.shape[-1]})")
-    if teacher_logits.device != logits.device or teacher_indices.device != logits.device:
-        raise RuntimeError("the teacher's tensors must be on the device of logits")
+    _check_gpu(logits, "logits")
     if not 1e-30 < temperature < 1e30:
         raise ValueError(f"temperature must be positive and finite (got {temperature})")
     _native.ensure()
-    loss, _state, _count = _topk_distill_fwd(logits, teacher_logits, teacher_indices, float(temperature))
+    loss, _state = _topk_distill_fwd(logits, teacher_logits, teacher_indices, float(temperature))
     return loss
 
 
@@ -368,9 +387,9 @@ _LIB.define("rope_fwd(Tensor query, Tensor key, Tensor cos, Tensor sin, bool inv
 _LIB.define("topk_sample(Tensor logits, Tensor noise, SymInt k) -> Tensor")
 _LIB.define("topk_verify(Tensor logits, Tensor? draft_logits, Tensor tokens, Tensor parents, Tensor uniform, Tensor noise, "
             "SymInt k) -> (Tensor, Tensor, Tensor)")
-# (loss fp32 scalar, row state fp32 [rows, 4], rows with entries fp32 scalar); the last two feed the backward
-_LIB.define("topk_distill_fwd(Tensor logits, Tensor teacher, Tensor index, float temperature) -> (Tensor, Tensor, Tensor)")
-_LIB.define("topk_distill_bwd(Tensor logits, Tensor teacher, Tensor index, Tensor row_state, Tensor count, Tensor grad, "
+# (loss fp32 scalar, row state fp32 [rows + 1, 4], which feeds the backward)
+_LIB.define("topk_distill_fwd(Tensor logits, Tensor teacher, Tensor index, float temperature) -> (Tensor, Tensor)")
+_LIB.define("topk_distill_bwd(Tensor logits, Tensor teacher, Tensor index, Tensor row_state, Tensor grad, "
             "float temperature) -> Tensor")
 
 
@@ -450,6 +469,7 @@ def _topk_sample_fake(logits, noise, k):
 
 @torch.library.register_fake("mega_trading_amd::topk_verify")
 def _topk_verify_fake(logits, draft_logits, tokens, parents, uniform, noise, k):
+    _check_verify(logits, draft_logits, tokens, parents, uniform, noise, k)
     b, n = tokens.shape
     return (tokens.new_empty((b, n), dtype=torch.int32), tokens.new_empty((b,), dtype=torch.int32),
             tokens.new_empty((b, 1)))
@@ -457,13 +477,13 @@ def _topk_verify_fake(logits, draft_logits, tokens, parents, uniform, noise, k):
 
 @torch.library.register_fake("mega_trading_amd::topk_distill_fwd")
 def _topk_distill_fwd_fake(logits, teacher, index, temperature):
+    _check_distillation(logits, teacher, index)
     f32 = dict(dtype=torch.float32)
-    return (logits.new_empty((), **f32), logits.new_empty((logits.numel() // logits.shape[-1], 4), **f32),
-            logits.new_empty((), **f32))
+    return logits.new_empty((), **f32), logits.new_empty((logits.numel() // logits.shape[-1] + 1, 4), **f32)
 
 
 @torch.library.register_fake("mega_trading_amd::topk_distill_bwd")
-def _topk_distill_bwd_fake(logits, teacher, index, row_state, count, grad, temperature):
+def _topk_distill_bwd_fake(logits, teacher, index, row_state, grad, temperature):
     return _like(logits)
 
 

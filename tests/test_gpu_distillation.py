@@ -89,7 +89,7 @@ def test_rows_without_entries(mta):
     assert mta.ops.topk_distillation(leaf, torch.full_like(y, -math.inf).to(DEV), i.to(DEV)).item() == 0.0
     empty = torch.zeros(0, 33, device=DEV, requires_grad=True)
     loss = mta.ops.topk_distillation(empty, torch.zeros(0, 5, device=DEV), torch.zeros(0, 5, dtype=torch.int64, device=DEV))
-    assert float(loss) == 0.0 and torch.autograd.grad(loss, empty)[0].shape == (0, 33)
+    assert loss.item() == 0.0 and torch.autograd.grad(loss, empty)[0].shape == (0, 33)
 
 
 def test_one_entry_is_cross_entropy(mta):

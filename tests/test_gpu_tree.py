@@ -16,6 +16,7 @@ import pytest
 import torch
 
 from oracle import tree_oracle as orc
+from tests import tree_refusals as refusals
 
 pytestmark = pytest.mark.gpu
 
@@ -75,6 +76,14 @@ def check_attention(out, q, k, v, kc, vc, lengths, parents, name=""):
             bound = bound + 2.0 ** -25  # half a step among the subnormals
         worst = float((abs(got[i] - ref) / bound).max())
         assert worst <= 1.0, f"{name} sequence {i} (length {n}): error {worst:.2f} of its bound"
+
+
+@pytest.mark.parametrize("cases", [refusals.tree_attention, refusals.tree_rope_and_commit, refusals.topk_verify,
+                                   refusals.topk_distillation], ids=lambda f: f.__name__)
+def test_refusals_before_any_launch(mta, cases):
+    for err, match, call in cases(mta):
+        with pytest.raises(err, match=match):
+            call()
 
 
 # ---------------------------------------------------------------------------

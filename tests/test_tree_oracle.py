@@ -12,6 +12,7 @@ import torch.nn.functional as F
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 from oracle import tree_oracle as orc
+from tests import tree_refusals as refusals
 
 BF16 = torch.bfloat16
 
@@ -85,117 +86,43 @@ def test_distillation_against_autograd():
 # ---------------------------------------------------------------------------
 # refusals: nothing is launched
 # ---------------------------------------------------------------------------
+@pytest.mark.parametrize("cases", [refusals.tree_attention, refusals.tree_rope_and_commit, refusals.topk_verify,
+                                   refusals.topk_distillation], ids=lambda f: f.__name__)
+def test_refusals(mta, cases):
+    with FakeTensorMode():
+        for err, match, call in cases(mta):
+            with pytest.raises(err, match=match):
+                call()
+
+
 def _fake(*shape, dtype=BF16):
     return torch.empty(*shape, device="cuda", dtype=dtype)
 
 
-def _nodes(n=5, hq=4, hkv=2, d=64, b=2, cap=32, dtype=BF16):
-    return [_fake(b, h, m, d, dtype=dtype) for h, m in ((hq, n), (hkv, n), (hkv, n), (hkv, cap), (hkv, cap))]
-
-
-def test_tree_attention_refuses(mta):
+def test_traced_calls_have_the_results_shapes(mta):
     with FakeTensorMode():
-        par = _fake(5, dtype=torch.int32)
-        args = _nodes()
-        assert mta.tree_attention(*args, 7, par, repeats=2).shape == args[0].shape
-        assert mta.tree_attention(*args, _fake(2, dtype=torch.int32), _fake(2, 5, dtype=torch.int32), repeats=2).shape == args[0].shape
-        for err, match, call in (
-            (RuntimeError, "unsupported dtype", lambda: mta.tree_attention(*_nodes(dtype=torch.float32), 7, par, repeats=2)),
-            (ValueError, "1 to 64 nodes", lambda: mta.tree_attention(*_nodes(n=65), 7, _fake(65, dtype=torch.int32), repeats=2)),
-            (ValueError, "1 to 64 nodes", lambda: mta.tree_attention(*_nodes(n=0), 7, _fake(0, dtype=torch.int32), repeats=2)),
-            (ValueError, "head_dim must be one of", lambda: mta.tree_attention(*_nodes(d=48), 7, par, repeats=2)),
-            (ValueError, "multiplied by repeats", lambda: mta.tree_attention(*args, 7, par, repeats=4)),
-            (ValueError, "positive multiple", lambda: mta.tree_attention(*_nodes(hq=3), 7, par, repeats=2)),
-            (ValueError, "outside", lambda: mta.tree_attention(*args, 33, par, repeats=2)),
-            (ValueError, "outside", lambda: mta.tree_attention(*args, -1, par, repeats=2)),
-            (ValueError, "tensor length", lambda: mta.tree_attention(*args, _fake(3, dtype=torch.int32), par, repeats=2)),
-            (ValueError, "tensor length", lambda: mta.tree_attention(*args, _fake(2, dtype=torch.int64), par, repeats=2)),
-            (ValueError, "parents must be int32", lambda: mta.tree_attention(*args, 7, _fake(5, dtype=torch.int64), repeats=2)),
-            (ValueError, "parents must be int32", lambda: mta.tree_attention(*args, 7, _fake(4, dtype=torch.int32), repeats=2)),
-            (ValueError, "agree on batch", lambda: mta.tree_attention(args[0], *_nodes(n=6)[1:3], *args[3:], 7, par, repeats=2)),
-            (ValueError, "caches must have the batch", lambda: mta.tree_attention(*args[:3], *_nodes(b=3)[3:], 7, par, repeats=2)),
-            (RuntimeError, "caches must have the dtype", lambda: mta.tree_attention(*args[:3], *_nodes(dtype=torch.float16)[3:], 7, par, repeats=2)),
-        ):
-            with pytest.raises(err, match=match):
-                call()
-    x = torch.zeros(1, 2, 3, 64)
-    with pytest.raises(RuntimeError, match="ROCm GPU"):
-        mta.tree_attention(x, x, x, x, x, 1, torch.zeros(3, dtype=torch.int32), repeats=1)
-
-
-def test_tree_rope_and_commit_refuse(mta):
-    with FakeTensorMode():
-        q, k, v, kc, vc = _nodes()
-        par, cs = _fake(5, dtype=torch.int32), _fake(1, 1, 16, 32, dtype=torch.float32)
-        path, count = _fake(2, 5, dtype=torch.int32), _fake(2, dtype=torch.int32)
+        q, k, v, kc, vc = refusals._nodes()
+        par, length, cs = _fake(5, dtype=torch.int32), _fake(2, dtype=torch.int32), _fake(1, 1, 16, 32, dtype=torch.float32)
+        assert mta.tree_attention(q, k, v, kc, vc, 7, par, repeats=2).shape == q.shape
+        assert mta.tree_attention(q, k, v, kc, vc, length, par.expand(2, 5), repeats=2).shape == q.shape
         assert [t.shape for t in mta.tree_rope(q, k, cs, cs, 15, par)] == [q.shape, k.shape]
-        mta.tree_commit([k], [v], path, count, 3, [kc], [vc])
-        for err, match, call in (
-            (ValueError, "outside", lambda: mta.tree_rope(q, k, cs, cs, 16, par)),
-            (ValueError, "head_dim/2", lambda: mta.tree_rope(q, k, cs[..., :31], cs, 3, par)),
-            (ValueError, "multiple of 8", lambda: mta.tree_rope(_fake(2, 4, 5, 20), _fake(2, 2, 5, 20), cs, cs, 3, par)),
-            (ValueError, "must have rows", lambda: mta.tree_rope(q, k, cs[:, :, :0], cs, 0, par)),
-            (ValueError, "one tensor per layer", lambda: mta.tree_commit([], [], path, count, 3, [], [])),
-            (ValueError, "one tensor per layer", lambda: mta.tree_commit([k, k], [v], path, count, 3, [kc], [vc])),
-            (ValueError, "share one shape", lambda: mta.tree_commit([k], [v[:, :, :4]], path, count, 3, [kc], [vc])),
-            (ValueError, "path must be int32", lambda: mta.tree_commit([k], [v], path.long(), count, 3, [kc], [vc])),
-            (ValueError, "count must be int32", lambda: mta.tree_commit([k], [v], path, _fake(2, 1, dtype=torch.int32), 3, [kc], [vc])),
-            (ValueError, "unit last-dim", lambda: mta.tree_commit([k], [v], path, count, 3, [_fake(2, 2, 64, 32).transpose(2, 3)], [vc])),
-            (ValueError, "same shape", lambda: mta.tree_commit([k], [v], path, count, 3, [kc], [vc[:, :, :9]])),
-            (RuntimeError, "dtype and device", lambda: mta.tree_commit([k], [v], path, count, 3, [kc.half()], [vc.half()])),
-            (RuntimeError, "unsupported dtype", lambda: mta.tree_commit([k.float()], [v.float()], path, count, 3, [kc.float()], [vc.float()])),
-        ):
-            with pytest.raises(err, match=match):
-                call()
-
-
-def test_topk_verify_refuses(mta):
-    with FakeTensorMode():
-        x, tok, par = _fake(2, 5, 40), _fake(2, 5, dtype=torch.int64), _fake(2, 5, dtype=torch.int32)
-        u, e = _fake(2, 5, dtype=torch.float32), _fake(2, 40, dtype=torch.float32)
-        out = mta.ops.topk_verify(x, tok, par, u, e, 8, draft_logits=x)
+        path, count = _fake(2, 5, dtype=torch.int32), _fake(2, dtype=torch.int32)
+        assert mta.tree_commit([k], [v], path, count, 3, [kc], [vc]) is None
+        x, tok = _fake(2, 5, 40), _fake(2, 5, dtype=torch.int64)
+        out = mta.ops.topk_verify(x, tok, par, _fake(2, 5, dtype=torch.float32), _fake(2, 40, dtype=torch.float32), 8,
+                                  draft_logits=x)
         assert [(tuple(t.shape), t.dtype) for t in out] == [((2, 5), torch.int32), ((2,), torch.int32), ((2, 1), torch.int64)]
-        f = mta.ops.topk_verify
-        for err, match, call in (
-            (ValueError, "1 <= k <= vocab", lambda: f(x, tok, par, u, e, 0)),
-            (ValueError, "1 <= k <= vocab", lambda: f(x, tok, par, u, e, 41)),
-            (ValueError, "32768", lambda: f(_fake(2, 5, 32769), tok, par, u, _fake(2, 32769, dtype=torch.float32), 8)),
-            (ValueError, "1 to 64 nodes", lambda: f(_fake(2, 65, 40), tok, par, u, e, 8)),
-            (ValueError, r"\[batch, nodes, vocab\]", lambda: f(x[0], tok, par, u, e, 8)),
-            (ValueError, "tokens must be", lambda: f(x, tok.int(), par, u, e, 8)),
-            (ValueError, "parents must be", lambda: f(x, tok, par.long(), u, e, 8)),
-            (ValueError, "uniform must be", lambda: f(x, tok, par, u[:, :4], e, 8)),
-            (ValueError, "noise must be", lambda: f(x, tok, par, u, e.double(), 8)),
-            (ValueError, "shape of logits", lambda: f(x, tok, par, u, e, 8, draft_logits=x[:, :4])),
-            (RuntimeError, "dtype and device", lambda: f(x, tok, par, u, e, 8, draft_logits=x.float())),
-            (RuntimeError, "unsupported", lambda: f(x.double(), tok, par, u, e, 8)),
-        ):
-            with pytest.raises(err, match=match):
-                call()
+        y, i = _fake(2, 5, 7, dtype=torch.float32), _fake(2, 5, 7, dtype=torch.int64)
+        assert mta.ops.topk_distillation(x, y, i, temperature=2.0).shape == ()
 
 
-def test_topk_distillation_refuses(mta):
-    with FakeTensorMode():
-        x, y, i = _fake(2, 3, 40), _fake(2, 3, 7, dtype=torch.float32), _fake(2, 3, 7, dtype=torch.int64)
-        f = mta.ops.topk_distillation
-        assert f(x, y, i, temperature=2.0).shape == ()
-        for err, match, call in (
-            (ValueError, "rows of logits", lambda: f(x, y[:1], i[:1])),
-            (ValueError, "rows of logits", lambda: f(x, y[0], i[0])),
-            (ValueError, "shape of teacher_logits", lambda: f(x, y, i[..., :6])),
-            (ValueError, "integer tensor", lambda: f(x, y, y)),
-            (ValueError, "1 to 1024", lambda: f(x, _fake(2, 3, 1025), _fake(2, 3, 1025, dtype=torch.int64))),
-            (ValueError, "1 to 1024", lambda: f(x, y[..., :0], i[..., :0])),
-            (ValueError, "temperature", lambda: f(x, y, i, temperature=0.0)),
-            (ValueError, "temperature", lambda: f(x, y, i, temperature=math.nan)),
-            (ValueError, "temperature", lambda: f(x, y, i, temperature=math.inf)),
-            (RuntimeError, "unsupported", lambda: f(x.double(), y, i)),
-            (RuntimeError, "unsupported", lambda: f(x, y.double(), i)),
-        ):
-            with pytest.raises(err, match=match):
-                call()
-    with pytest.raises(RuntimeError, match="ROCm GPU"):
-        f(torch.zeros(2, 4), torch.zeros(2, 1), torch.zeros(2, 1, dtype=torch.int64))
+def test_cpu_tensors_are_refused(mta):
+    x, n = torch.zeros(1, 2, 3, 64), torch.zeros(3, dtype=torch.int32)
+    for call in (lambda: mta.tree_attention(x, x, x, x, x, 1, n, repeats=1), lambda: mta.tree_rope(x, x, x, x, 1, n),
+                 lambda: mta.tree_commit([x], [x], n, n, 1, [x], [x]),
+                 lambda: mta.ops.topk_verify(x, n, n, n, n, 1), lambda: mta.ops.topk_distillation(x, x, n)):
+        with pytest.raises(RuntimeError, match="ROCm GPU"):
+            call()
 
 
 def test_c_entry_points_refuse(mta):
@@ -245,13 +172,13 @@ def test_c_entry_points_refuse(mta):
     assert verify(b=0) == 0
 
     def distill(x=p, ld=40, rows=3, v=40, k=7, t=1.0, state=p, dt=0):
-        return lib.mt_topk_distill_fwd(x, ld, p, p, rows, v, k, t, state, p, p, dt, None)
+        return lib.mt_topk_distill_fwd(x, ld, p, p, rows, v, k, t, state, p, dt, None)
 
     assert distill(dt=3) == E_DTYPE and distill(ld=39) == E_STRIDE and distill(rows=-1) == E_SHAPE and distill(v=0) == E_SHAPE
     assert distill(k=0) == E_SHAPE and distill(k=1025) == E_SHAPE and distill(t=0.0) == E_SHAPE and distill(t=math.inf) == E_SHAPE
     assert distill(x=None) == E_NULL and distill(x=p + 1) == E_STRIDE and distill(state=p + 4) == E_STRIDE
-    assert lib.mt_topk_distill_bwd(p, 40, p, p, p, p, None, p, 3, 40, 7, 1.0, 0, None) == E_NULL
-    assert lib.mt_topk_distill_bwd(None, 40, None, None, None, None, None, None, 0, 40, 7, 1.0, 0, None) == 0
+    assert lib.mt_topk_distill_bwd(p, 40, p, p, p, None, p, 3, 40, 7, 1.0, 0, None) == E_NULL
+    assert lib.mt_topk_distill_bwd(None, 40, None, None, None, None, None, 0, 40, 7, 1.0, 0, None) == 0
 
 
 # ---------------------------------------------------------------------------
@@ -285,8 +212,8 @@ def test_distillation_gradient_rules(mta):
     mta._native.load()
     ops = torch.ops.mega_trading_amd
     x, y, i = _meta(3, 9, dtype=BF16, grad=True), _meta(3, 4, grad=True), _meta(3, 4, dtype=torch.int64)
-    loss, state, count = ops.topk_distill_fwd(x, y, i, 2.0)
-    assert loss.requires_grad and not state.requires_grad and not count.requires_grad
+    loss, state = ops.topk_distill_fwd(x, y, i, 2.0)
+    assert loss.requires_grad and not state.requires_grad
     gx, gy = torch.autograd.grad(loss, (x, y), allow_unused=True, create_graph=True)
     assert gx.shape == x.shape and gx.dtype == BF16 and gy is None
     with pytest.raises(RuntimeError, match="no autograd formula"):
