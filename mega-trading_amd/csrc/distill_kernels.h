@@ -10,8 +10,13 @@
 //
 // Bound by memory: the forward reads each logit once (a running maximum and sum), the
 // backward reads it and writes its gradient once.  One workgroup of 256 threads a row,
-// 8 values a lane a step; rows need no alignment beyond their type's (an odd
-// vocabulary), since a global load of 16 bytes takes any address.
+// 8 values a load, kDistillAhead loads of a thread in flight; rows need no alignment
+// beyond their type's (an odd vocabulary), since a global load of 16 bytes takes any
+// address.  The backward starts with the rows that the forward read last: part of them
+// is still in the 256 MB cache in front of the memory (688 -> 670 us for the step).
+//
+// 32768 rows of 16384 bf16 logits, 64 entries: forward 178 us (6.0 TB/s), its sum 10,
+// backward 426 (5.0 TB/s read and written, what a large copy reaches).
 #pragma once
 
 #include "storage.h"
@@ -109,9 +114,9 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams a) {
       s *= exp2_fast((m - mx) * c2);
       m = mx;
     }
-    if (m == -INFINITY) return;
+    const float from = m == -INFINITY ? 0.f : m;  // before any number: -inf adds 0, NaN stays NaN
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s += exp2_fast((v[j] - m) * c2);
+    for (int j = 0; j < 8; ++j) s += exp2_fast((v[j] - from) * c2);
   };
   const int nvec = a.V / 8;
   for (int c0 = tid; c0 < nvec; c0 += 256 * kDistillAhead) {
@@ -153,12 +158,12 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams a) {
 __global__ __launch_bounds__(1024) void distill_sum_kernel(float* row, int64_t rows, float t2, float* loss) {
   __shared__ double part[2][16];
   double s = 0., n = 0.;
-  for (int64_t i = threadIdx.x; i < rows; i += 8 * 1024) {
-    f32x4 v[8];
+  for (int64_t i = threadIdx.x; i < rows; i += 16 * 1024) {
+    f32x4 v[16];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const f32x4*>(row + 4 * min(i + 1024 * j, rows - 1));
+    for (int j = 0; j < 16; ++j) v[j] = *reinterpret_cast<const f32x4*>(row + 4 * min(i + 1024 * j, rows - 1));
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < 16; ++j)
       if (i + 1024 * j < rows) {
         s += v[j][0];
         n += v[j][3];
@@ -184,19 +189,20 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(float* row, int64_t r
   }
 }
 
-template <int DT>
+// PAST: the gradient goes past the caches.
+template <int DT, bool PAST>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
   __shared__ float buf[4];
   __shared__ int64_t idx[kDistillEntries];
   __shared__ float prob[kDistillEntries];
-  const int64_t row = blockIdx.x;
+  const int64_t row = a.rows - 1 - blockIdx.x;  // the rows that the forward read last first: some are still in a cache
   const int tid = threadIdx.x;
   const int64_t base = row * a.ldx, out = row * a.V;
   const int nvec = a.V / 8;
   const f32x4 r = *reinterpret_cast<const f32x4*>(a.row + 4 * row);
   if (r[3] == 0.f) {
     const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int c = tid; c < nvec; c += 256) ops::store8_any<DT>(a.dx, out + 8 * c, z);
+    for (int c = tid; c < nvec; c += 256) ops::store8_any<DT, PAST>(a.dx, out + 8 * c, z);
     if (tid < a.V - 8 * nvec) ops::IO<DT>::store1(a.dx, out + 8 * nvec + tid, 0.f);
     return;
   }
@@ -224,7 +230,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
       ops::IO<DT>::unpack(r[i], v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = exp2_fast((v[j] - M) * c2) * qs;
-      ops::store8_any<DT>(a.dx, out + 8 * (c0 + 256 * i), v);
+      ops::store8_any<DT, PAST>(a.dx, out + 8 * (c0 + 256 * i), v);
     }
   }
   if (tid < a.V - 8 * nvec) {

@@ -345,7 +345,11 @@ int mt_tree_commit(const void* const* keys, const void* const* values, void* con
       p.dst[0][l] = static_cast<uint16_t*>(key_caches[l0 + l]);
       p.dst[1][l] = static_cast<uint16_t*>(value_caches[l0 + l]);
     }
-    const int64_t n = (int64_t)N * p.layers * 2 * Hkv * (wide ? D / 8 : D), blocks = (n + 255) / 256;
+    // The nodes are shared out while that takes no more than 4 workgroups a CU (8 layers, 4 trees of 64 nodes,
+    // 8 heads of 128: 24 us with one thread a node, 13.5 with up to 2 workgroups a CU, 11.3 with 4, 11.5 with 8).
+    const int64_t n = (int64_t)p.layers * 2 * Hkv * (wide ? D / 8 : D);
+    p.split = (int)std::max<int64_t>(1, std::min<int64_t>(N, 4 * (int64_t)device_cus() * 256 / (n * B)));
+    const int64_t blocks = (n * p.split + 255) / 256;
     if (blocks * B > 0x7fffffffLL) return fail(MT_E_SHAPE, "too many values");
     p.blocks = (int)blocks;
     const dim3 grid((unsigned)(blocks * B));
@@ -480,9 +484,16 @@ int mt_topk_distill_bwd(const void* logits, int64_t row_stride, const float* tea
   p.dx = dlogits;
   const dim3 grid((unsigned)rows);
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == MT_DTYPE_BF16) hipLaunchKernelGGL((mt::distill_bwd_kernel<kDtBF16>), grid, dim3(256), 0, st, p);
-  else if (dtype == MT_DTYPE_FP16) hipLaunchKernelGGL((mt::distill_bwd_kernel<kDtFP16>), grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((mt::distill_bwd_kernel<kDtFP32>), grid, dim3(256), 0, st, p);
+  // A gradient larger than the 256 MB cache in front of the memory cannot stay there: stored past it, it
+  // leaves the logits (32768 x 16384 bf16: 452 + 217 us with the forward of the next step, 424 + 201 past it).
+  const bool past = rows * vocab * (dtype == MT_DTYPE_FP32 ? 4 : 2) > int64_t(256) << 20;
+#define MT_DISTILL_BWD(DT)                                                                        \
+  if (past) hipLaunchKernelGGL((mt::distill_bwd_kernel<DT, true>), grid, dim3(256), 0, st, p);    \
+  else hipLaunchKernelGGL((mt::distill_bwd_kernel<DT, false>), grid, dim3(256), 0, st, p)
+  if (dtype == MT_DTYPE_BF16) { MT_DISTILL_BWD(kDtBF16); }
+  else if (dtype == MT_DTYPE_FP16) { MT_DISTILL_BWD(kDtFP16); }
+  else { MT_DISTILL_BWD(kDtFP32); }
+#undef MT_DISTILL_BWD
   return launched("distillation");
 }
 

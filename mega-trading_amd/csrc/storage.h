@@ -104,18 +104,23 @@ __device__ __forceinline__ typename IO<DT>::Raw load8_any(const void* base, int6
   if constexpr (DT == kDtFP32) r.w[1] = p[1];
   return r;
 }
-template <int DT>
+// PAST: past the caches, for what is too large to stay in them
+template <bool PAST>
+__device__ __forceinline__ void put16(u32x4_any* p, u32x4 v) {
+  if constexpr (PAST) __builtin_nontemporal_store((u32x4_any)v, p);
+  else *p = v;
+}
+template <int DT, bool PAST = false>
 __device__ __forceinline__ void store8_any(void* base, int64_t i, const float* v) {
   u32x4_any* p = reinterpret_cast<u32x4_any*>(static_cast<char*>(base) + i * (DT == kDtFP32 ? 4 : 2));
   if constexpr (DT == kDtFP32) {
-    p[0] = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-    p[1] = u32x4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
+    put16<PAST>(p, u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])});
+    put16<PAST>(p + 1, u32x4{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])});
   } else {
     using E = typename std::conditional<DT == kDtBF16, BF16, FP16>::type;
-    p[0] = u32x4{pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3]), pack2<E>(v[4], v[5]), pack2<E>(v[6], v[7])};
+    put16<PAST>(p, u32x4{pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3]), pack2<E>(v[4], v[5]), pack2<E>(v[6], v[7])});
   }
 }
-
 
 }  // namespace ops
 }  // namespace mt

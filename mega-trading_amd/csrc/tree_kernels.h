@@ -630,8 +630,8 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(TreeAttnParams p) {
 
 // ===========================================================================
 // Accepted nodes into the caches: cache[b, h, cached(b) + j] = node[b, h, path[b, j]]
-// for j < count[b], keys and values of up to kCommitLayers layers in one launch.  One thread
-// per W 16-bit values; slots j >= count end at once, j the slowest index.
+// for j < count[b], keys and values of up to kCommitLayers layers in one launch.  A thread takes W
+// 16-bit values of one (layer, key or value, head) and every split-th node, four of them in flight.
 // ===========================================================================
 constexpr int kCommitLayers = 32;
 
@@ -642,12 +642,15 @@ struct TreeCommitParams {
   const int *path, *count;                // [B, N], [B]
   TreeShape t;                            // parents unused
   int layers, Hkv, D;
+  int split;   // threads that share a (layer, key or value, head, values)
   int blocks;  // workgroups of a sequence
 };
 
 template <int W>
 __global__ __launch_bounds__(256) void tree_commit_kernel(TreeCommitParams p) {
-  const int b = blockIdx.x / p.blocks, nc = p.D / W;
+  using V = typename std::conditional<W == 8, u32x4, uint16_t>::type;
+  constexpr int AHEAD = 4;
+  const int b = blockIdx.x / p.blocks, nc = p.D / W, N = p.t.N;
   int64_t i = (int64_t)(blockIdx.x % p.blocks) * 256 + threadIdx.x;
   const int c = int(i % nc);
   i /= nc;
@@ -655,15 +658,25 @@ __global__ __launch_bounds__(256) void tree_commit_kernel(TreeCommitParams p) {
   i /= p.Hkv;
   const int w = int(i % 2);
   i /= 2;
-  const int layer = int(i % p.layers);
-  const int j = int(i / p.layers);
-  if (j >= min(p.count[b], p.t.N)) return;
-  const int node = p.path[(int64_t)b * p.t.N + j], pos = p.t.cached(b) + j;
-  if (node < 0 || node >= p.t.N || pos >= p.t.capacity) return;
-  const uint16_t* s = p.src[w][layer] + b * p.ss[w][0] + (int64_t)h * p.ss[w][1] + (int64_t)node * p.ss[w][2] + W * c;
-  uint16_t* d = p.dst[w][layer] + b * p.sd[w][0] + (int64_t)h * p.sd[w][1] + (int64_t)pos * p.sd[w][2] + W * c;
-  if constexpr (W == 8) *reinterpret_cast<u32x4*>(d) = *reinterpret_cast<const u32x4*>(s);
-  else *d = *s;
+  const int layer = int(i % p.layers), first = int(i / p.layers);
+  if (first >= p.split) return;
+  const uint16_t* src = p.src[w][layer] + b * p.ss[w][0] + (int64_t)h * p.ss[w][1] + W * c;
+  uint16_t* dst = p.dst[w][layer] + b * p.sd[w][0] + (int64_t)h * p.sd[w][1] + W * c;
+  const int cached = p.t.cached(b), count = min(p.count[b], min(N, p.t.capacity - cached));
+  for (int j0 = first; j0 < count; j0 += AHEAD * p.split) {
+    int node[AHEAD];
+    V x[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) node[a] = p.path[(int64_t)b * N + min(j0 + a * p.split, N - 1)];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a)
+      x[a] = *reinterpret_cast<const V*>(src + (int64_t)min(max(node[a], 0), N - 1) * p.ss[w][2]);
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int j = j0 + a * p.split;
+      if (j < count && node[a] >= 0 && node[a] < N) *reinterpret_cast<V*>(dst + (int64_t)(cached + j) * p.sd[w][2]) = x[a];
+    }
+  }
 }
 
 }  // namespace mt

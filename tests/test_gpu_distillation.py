@@ -130,6 +130,21 @@ def test_an_index_past_the_vocabulary_spoils_its_row_alone(mta):
     assert math.isnan(float(loss)) and grad[[0, 2, 3, 4]].isfinite().all() and grad[1].isnan().any()
 
 
+@pytest.mark.parametrize("where", [slice(8, 16), slice(1000, 1001), slice(3, 4), slice(0, 1001)])
+def test_a_logit_that_is_no_number_spoils_its_row_alone(mta, where):
+    # alone in a thread, whole vectors of them, and beside -inf: the softmax over such a row is NaN everywhere
+    x, y, i = inputs(4, 1001, 8, BF16, 15)
+    x[1, where] = math.nan
+    x[2, :] = -math.inf
+    x[2, where] = math.nan
+    i[1:3] = 500
+    leaf = x.to(DEV).requires_grad_(True)
+    loss = mta.ops.topk_distillation(leaf, y.to(DEV), i.to(DEV))
+    grad, = torch.autograd.grad(loss, leaf)
+    assert math.isnan(float(loss)) and grad[1:3].isnan().all() and grad[[0, 3]].isfinite().all()
+    assert math.isnan(float(mta.ops.topk_distillation(x[1:2].to(DEV), y[1:2].to(DEV), i[1:2].to(DEV))))
+
+
 def test_layouts_and_types_of_the_teacher(mta):
     x, y, i = inputs(12, 101, 8, BF16, 5)
     ref = check(mta, x, y.to(BF16), i, 2.0)
