@@ -89,19 +89,34 @@ struct Split {
   int64_t nspan;
 };
 Split split(int64_t B, int64_t Hkv, int64_t R, int N, int64_t cached, int D) {
-  Split s;
-  const int64_t rows = R * N;
-  s.rw = rows <= 32 ? 0 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
-  const int take = s.rw ? 32 * s.rw : 32, waves = D == 128 ? 8 : 16;
+  Split s{};
+  const int64_t rows = R * N, cus = device_cus(), tiles32 = (cached + 31) / 32 + (N + 31) / 32;
+  // The smallest row blocks that still give no CU two workgroups (a workgroup fills a CU): more CUs work, and a
+  // workgroup's tiles go to more key groups.  But every block reads all keys, which counts when there are many of
+  // them: up to 96 tiles of 32 keys a CU for blocks of 32 rows (32 at D = 128), 4 times that for blocks of
+  // twice the rows.  us at blocks of 32 / 64 / 128 / 256 rows, span joins included; KV heads of all sequences, rows
+  // of each, D, keys:
+  //    64,  64,  64,   545:  8.4 / 12.3                    16, 256,  64, 10000:  31.3 / 26.3 / 28.4 / 37.9
+  //    64, 128,  64,  1000: 11.5 / 14.8 / 20.5             64, 256,  64,  1000:  21.8 / 16.2 / 23.8 / 29.8
+  //   128, 256,  64,  3000: 73.0 / 48.6 / 41.9 / 53.4     256, 256,  64, 10000:   377 /  286 /  259 /  231
+  //    16, 128, 128,  1000: 15.4 / 15.9 / 19.6             64, 128, 128,  3000:  36.9 / 31.0 / 33.7
+  //    64, 128, 128, 10000:  105 / 82.6 / 71.3             64, 256, 128,   300:  22.9 / 12.7 / 26.0 / 35.1
+  int64_t most_tiles = (D == 128 ? 32 : 96) * cus;
+  int take = 32;
+  for (;; take *= 2, most_tiles *= 4) {
+    s.blocks = (int)((rows + take - 1) / take);
+    const int64_t n = B * Hkv * s.blocks;
+    if (s.blocks == 1 || take == 256 || (n <= cus && n * tiles32 <= most_tiles)) break;
+  }
+  const int waves = D == 128 ? 8 : 16;
+  s.rw = take == 32 ? 0 : take / 32;
   s.keys = s.rw ? 16 * s.rw : mt::kTreeKeys;
   s.groups = s.rw ? waves / s.rw : waves / 2;
-  s.blocks = (int)((rows + take - 1) / take);
   const int64_t tiles = (cached + s.keys - 1) / s.keys + (N + s.keys - 1) / s.keys;
-  // A workgroup fills a CU.  Up to 192 keys a key group stay with one workgroup: joining spans is another
-  // launch (5 nodes on 200 of 1024 cached keys, 2 heads of 64: 6.5 us against 7.0 and 3.4; 16 nodes, 32 sequences
-  // of about 500: 12.9 against 11.9 and 3.5; 64 nodes there, 2 key groups: 26.0 against 20.6 and 5.5).  More are split over all
-  // CUs, down to two tiles.
-  const int64_t want = (int64_t)device_cus() / std::max<int64_t>(1, B * Hkv * s.blocks);
+  // Up to 192 keys a key group stay with one workgroup: joining spans is another launch (one span against
+  // several, 8 heads over 2 KV heads of 64: 5 nodes on 200 of 1024 keys 6.1 / 10.2 us; 32 sequences of 16 nodes on 545
+  // of 1024 keys 8.5 / 11.9, on 1500 keys 11.8 / 12.8).  More are split over all CUs, down to two tiles.
+  const int64_t want = cus / std::max<int64_t>(1, B * Hkv * s.blocks);
   const int64_t most = tiles * s.keys <= 192 * s.groups ? 1 : (tiles + 2 * s.groups - 1) / (2 * s.groups);
   s.nspan = std::max<int64_t>(1, std::min(want, most));
   return s;

@@ -37,13 +37,17 @@ __device__ __forceinline__ uint64_t shfl64(uint64_t x, int src) {
   return ((uint64_t)hi << 32) | lo;
 }
 
-// Lane n: the ancestors of node n and n itself, bit by bit; 0 for padding and for lanes past N.
-__device__ __forceinline__ uint64_t tree_ancestors(const TreeShape& t, int b, int lane) {
-  const int p = lane < t.N ? t.parents[(int64_t)b * t.parents_stride + lane] : -2;
+// Lane n: the parent of node n, -2 past the nodes.
+__device__ __forceinline__ int tree_parent(const TreeShape& t, int b, int lane) {
+  return lane < t.N ? t.parents[(int64_t)b * t.parents_stride + lane] : -2;
+}
+
+// Lane n, with its parent: the ancestors of node n and n itself, bit by bit; 0 for padding and for lanes
+// past N.  As many rounds as the deepest node asks for: 3 for a chain of 5.
+__device__ __forceinline__ uint64_t tree_ancestors(int p, int lane) {
   uint64_t seen = 1ull << lane;
   int up = p >= 0 && p < lane ? p : -1, bad = p != -1 && up < 0;
-#pragma unroll
-  for (int r = 0; r < 6; ++r) {
+  while (__ballot(up >= 0)) {
     const int src = up < 0 ? lane : up;
     const uint64_t s = shfl64(seen, src);
     const int b2 = __shfl(bad, src, 64), u2 = __shfl(up, src, 64);
@@ -78,7 +82,7 @@ __global__ __launch_bounds__(256) void tree_rope_kernel(TreeRopeParams p) {
   __shared__ int pos[kTreeNodes];
   const int b = blockIdx.x / p.blocks, tid = threadIdx.x;
   if (tid < 64) {
-    const uint64_t seen = tree_ancestors(p.t, b, tid);
+    const uint64_t seen = tree_ancestors(tree_parent(p.t, b, tid), tid);
     pos[tid] = seen ? min(p.t.cached(b) + __popcll(seen) - 1, p.table_rows - 1) : -1;
   }
   __syncthreads();
@@ -193,22 +197,32 @@ constexpr int tree_few_waves() { return D == 128 ? 4 : 8; }  // what the tiles l
 
 template <class E, int D>
 __global__ __launch_bounds__(64 * tree_few_waves<D>()) void tree_attn_kernel(TreeAttnParams p) {
-  constexpr int NT = 1, W = tree_few_waves<D>();
+  constexpr int W = tree_few_waves<D>();
   using V8 = typename E::v8;
   using TL = Tile<D>;
   constexpr int KT = D / 16, DT = D / 32, TILE = kTreeKeys * TL::RB;
   constexpr int COPIES = 2 * TILE / 1024;  // of a K and a V tile
   constexpr int C4 = D / 4;                // 16-byte chunks of an fp32 row
-  __shared__ __attribute__((aligned(1024))) char smem[W][2][2][TILE];  // then the waves' o [32 NT][D] fp32
-  __shared__ float wm[W][32 * NT], wl[W][32 * NT];
-  static_assert(sizeof(smem[0]) >= 32 * NT * D * 4, "a wave's o fits its tiles");
+  __shared__ __attribute__((aligned(1024))) char smem[W][2][2][TILE];  // then the waves' o [32][D] fp32
+  __shared__ float wm[W][32], wl[W][32];
+  static_assert(sizeof(smem[0]) >= 32 * D * 4, "a wave's o fits its tiles");
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // the row blocks of one (sequence, KV head, span) on one XCD (index mod 8), one after the other
   const int slot = blockIdx.x % (8 * p.blocks), g = blockIdx.x / (8 * p.blocks) * 8 + slot % 8, rb = slot / 8;
   if (g >= p.B * p.Hkv * p.nspan) return;
   const int s = g % p.nspan, pair = g / p.nspan, kvh = pair % p.Hkv, b = pair / p.Hkv;
-  const int L = p.t.cached(b), N = p.t.N, RN = p.R * N;
+  const int N = p.t.N, RN = p.R * N;
+  // the loads that nothing is needed for, together: parents, length and queries
+  const int up = tree_parent(p.t, b, lane);
+  const int row = rb * 32 + l32, rc = min(row, RN - 1), node = rc % N;
+  u32x4 qraw[KT];
+  {
+    const uint16_t* qr = p.q + b * p.sq[0] + (int64_t)(kvh * p.R + rc / N) * p.sq[1] + (int64_t)node * p.sq[2] + 8 * hh;
+#pragma unroll
+    for (int kk = 0; kk < KT; ++kk) qraw[kk] = *reinterpret_cast<const u32x4*>(qr + 16 * kk);
+  }
+  const int L = p.t.cached(b);
   const TreeTiles tl(L, N, p.nspan, kTreeKeys, W);
   if (s >= tl.spans) return;  // the combine does not read this span
   const int t0 = (s * W + wave) * tl.per, t1 = min(tl.all, t0 + tl.per);
@@ -228,33 +242,17 @@ __global__ __launch_bounds__(64 * tree_few_waves<D>()) void tree_attn_kernel(Tre
     }
   };
 
-  // the rows' queries (B operands) and what they see of the tree
-  const uint64_t anc = tree_ancestors(p.t, b, lane);
-  V8 qop[NT][KT];
-  uint64_t seen[NT];
+  // what the rows see of the tree, and their queries (B operands)
+  const uint64_t anc = tree_ancestors(up, lane), above = shfl64(anc, node), seen = row < RN ? above : 0ull;
+  V8 qop[KT];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int row = (rb * NT + nt) * 32 + l32, rc = min(row, RN - 1), node = rc % N;
-    const uint16_t* qr = p.q + b * p.sq[0] + (int64_t)(kvh * p.R + rc / N) * p.sq[1] + (int64_t)node * p.sq[2] + 8 * hh;
-    const uint64_t a = shfl64(anc, node);
-    seen[nt] = row < RN ? a : 0ull;
-#pragma unroll
-    for (int kk = 0; kk < KT; ++kk) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(qr + 16 * kk);
-      qop[nt][kk] = __builtin_bit_cast(V8, seen[nt] ? x : zero4());
-    }
-  }
+  for (int kk = 0; kk < KT; ++kk) qop[kk] = __builtin_bit_cast(V8, seen ? qraw[kk] : zero4());
   const uint64_t padding = ~__ballot(anc != 0ull);  // nodes whose keys and values are not read
 
-  f32x16 oacc[DT][NT];
-  float mrun[NT], lrun[NT];
+  f32x16 oacc[DT];
+  float mrun = kTreeNone, lrun = 0.f;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    mrun[nt] = kTreeNone;
-    lrun[nt] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) zero16(oacc[dt][nt]);
-  }
+  for (int dt = 0; dt < DT; ++dt) zero16(oacc[dt]);
   const int rbase = TL::row_base(lane);
   const TrBase tbase = TL::tr_base(lane);
   const float c2 = p.scale_log2;
@@ -276,78 +274,60 @@ __global__ __launch_bounds__(64 * tree_few_waves<D>()) void tree_attn_kernel(Tre
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
-    f32x16 st[NT];
+    f32x16 st;
 #pragma unroll
-    for (int kk = 0; kk < KT; ++kk) {
-      const V8 a = TL::template row_op<E>(kl, rbase, 0, kk);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) st[nt] = E::mfma(a, qop[nt][kk], kk == 0 ? f32x16{} : st[nt]);
-    }
+    for (int kk = 0; kk < KT; ++kk)
+      st = E::mfma(TL::template row_op<E>(kl, rbase, 0, kk), qop[kk], kk == 0 ? f32x16{} : st);
     if (n0 >= 0 || (t + 1) * kTreeKeys > L) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = 8 * (i >> 2) + 4 * hh + (i & 3);
-          const bool in = n0 >= 0 ? (seen[nt] >> (n0 + key)) & 1 : t * kTreeKeys + key < L;
-          st[nt][i] = in ? st[nt][i] : -INFINITY;
-        }
+      for (int i = 0; i < 16; ++i) {
+        const int key = 8 * (i >> 2) + 4 * hh + (i & 3);
+        const bool in = n0 >= 0 ? (seen >> (n0 + key)) & 1 : t * kTreeKeys + key < L;
+        st[i] = in ? st[i] : -INFINITY;
+      }
     }
-    V8 pk[NT][2];
-    float qs[NT];
+    V8 pk[2];
+    float qs;
     // P = 2^(S c2 - m) in 16 bits; the sums add the rounded values, the weights that P V uses
-    auto ex = [&](int nt) {
+    auto ex = [&]() {
       u32x4 w[2];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        w[i >> 2][i & 3] = pack2<E>(exp2_fast(__builtin_fmaf(st[nt][2 * i], c2, -mrun[nt])),
-                                    exp2_fast(__builtin_fmaf(st[nt][2 * i + 1], c2, -mrun[nt])));
+        w[i >> 2][i & 3] = pack2<E>(exp2_fast(__builtin_fmaf(st[2 * i], c2, -mrun)),
+                                    exp2_fast(__builtin_fmaf(st[2 * i + 1], c2, -mrun)));
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         s0 = E::sum2(w[0][i], s0);
         s1 = E::sum2(w[1][i], s1);
       }
-      qs[nt] = s0 + s1;
-      pk[nt][0] = __builtin_bit_cast(V8, w[0]);
-      pk[nt][1] = __builtin_bit_cast(V8, w[1]);
+      qs = s0 + s1;
+      pk[0] = __builtin_bit_cast(V8, w[0]);
+      pk[1] = __builtin_bit_cast(V8, w[1]);
     };
-    bool high = false;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      ex(nt);
-      high |= !(qs[nt] <= kSumLimit);
-    }
+    ex();
     // a P above 2^kRescaleSlack (or the first keys): that row's m is raised to its maximum.  Other
     // rows of the wave keep theirs, so a row's result does not depend on the rows beside it.
-    if (__builtin_amdgcn_ballot_w64(high)) {
+    if (__builtin_amdgcn_ballot_w64(!(qs <= kSumLimit))) {
+      float v = -INFINITY;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float v = -INFINITY;
+      for (int i = 0; i < 16; ++i) v = fmaxf(v, st[i]);
+      const bool raise = max_with_partner(qs <= kSumLimit ? 0.f : 1.f) > 0.f;
+      v = max_with_partner(v) * c2;
+      const float m = raise ? fmaxf(mrun, v) : mrun, alpha = exp2_fast(mrun - m);
+      mrun = m;
+      lrun *= alpha;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v = fmaxf(v, st[nt][i]);
-        const bool raise = max_with_partner(qs[nt] <= kSumLimit ? 0.f : 1.f) > 0.f;
-        v = max_with_partner(v) * c2;
-        const float m = raise ? fmaxf(mrun[nt], v) : mrun[nt], alpha = exp2_fast(mrun[nt] - m);
-        mrun[nt] = m;
-        lrun[nt] *= alpha;
+      for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) oacc[dt][nt][i] *= alpha;
-        ex(nt);
-      }
+        for (int i = 0; i < 16; ++i) oacc[dt][i] *= alpha;
+      ex();
     }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) lrun[nt] += qs[nt];
+    lrun += qs;
 #pragma unroll
     for (int k2 = 0; k2 < 2; ++k2)
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const V8 a = TL::template tr_op<E>(vl, tbase, k2, dt);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) oacc[dt][nt] = E::mfma(a, pk[nt][k2], oacc[dt][nt]);
-      }
+      for (int dt = 0; dt < DT; ++dt) oacc[dt] = E::mfma(TL::template tr_op<E>(vl, tbase, k2, dt), pk[k2], oacc[dt]);
     if (t + 2 < t1) {
       reads_done();
       stage(t + 2, buf);
@@ -357,32 +337,28 @@ __global__ __launch_bounds__(64 * tree_few_waves<D>()) void tree_attn_kernel(Tre
 
   // the wave's o, 16-byte chunk c of row r at slot c ^ (r mod C4)
   float* ow = reinterpret_cast<float*>(smem[wave]);
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = nt * 32 + l32;
-    const float l = sum_with_partner(lrun[nt]);
-    if (hh == 0) {
-      wm[wave][r] = seen[nt] ? mrun[nt] : kTreeNone;
-      wl[wave][r] = seen[nt] ? l : 0.f;  // padding: no weight anywhere
-    }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = dt * 8 + 2 * q + hh;
-        *reinterpret_cast<f32x4*>(ow + r * D + 4 * (c ^ (r % C4))) =
-            f32x4{oacc[dt][nt][4 * q], oacc[dt][nt][4 * q + 1], oacc[dt][nt][4 * q + 2], oacc[dt][nt][4 * q + 3]};
-      }
+  const float l = sum_with_partner(lrun);
+  if (hh == 0) {
+    wm[wave][l32] = seen ? mrun : kTreeNone;
+    wl[wave][l32] = seen ? l : 0.f;  // padding: no weight anywhere
   }
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = dt * 8 + 2 * q + hh;
+      *reinterpret_cast<f32x4*>(ow + l32 * D + 4 * (c ^ (l32 % C4))) =
+          f32x4{oacc[dt][4 * q], oacc[dt][4 * q + 1], oacc[dt][4 * q + 2], oacc[dt][4 * q + 3]};
+    }
   __syncthreads();
-  for (int i = tid; i < 32 * NT * C4; i += 64 * W) {
-    const int r = i / C4, c = i % C4, row = rb * NT * 32 + r;
-    if (row >= RN) continue;
-    tree_merge<E, D, W>(p, pair, s, row, c, [&](int w) { return wm[w][r]; }, [&](int w) { return wl[w][r]; },
-                                 [&](int w) {
-                                   return *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(smem[w]) + r * D +
-                                                                          4 * (c ^ (r % C4)));
-                                 });
+  for (int i = tid; i < 32 * C4; i += 64 * W) {
+    const int r = i / C4, c = i % C4, at = rb * 32 + r;
+    if (at >= RN) continue;
+    tree_merge<E, D, W>(p, pair, s, at, c, [&](int w) { return wm[w][r]; }, [&](int w) { return wl[w][r]; },
+                        [&](int w) {
+                          return *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(smem[w]) + r * D +
+                                                                 4 * (c ^ (r % C4)));
+                        });
   }
 }
 
@@ -408,7 +384,17 @@ __global__ __launch_bounds__(64 * tree_waves<D>()) void tree_attn_rows_kernel(Tr
   const int slot = blockIdx.x % (8 * p.blocks), g = blockIdx.x / (8 * p.blocks) * 8 + slot % 8, rb = slot / 8;
   if (g >= p.B * p.Hkv * p.nspan) return;
   const int s = g % p.nspan, pair = g / p.nspan, kvh = pair % p.Hkv, b = pair / p.Hkv;
-  const int L = p.t.cached(b), N = p.t.N, RN = p.R * N;
+  const int N = p.t.N, RN = p.R * N;
+  const int up = tree_parent(p.t, b, lane);
+  const int row = (rb * RW + rw) * 32 + l32, rc = min(row, RN - 1), node = rc % N;
+  const bool active = (rb * RW + rw) * 32 < RN;  // wave-uniform
+  u32x4 qraw[KT];
+  {
+    const uint16_t* qr = p.q + b * p.sq[0] + (int64_t)(kvh * p.R + rc / N) * p.sq[1] + (int64_t)node * p.sq[2] + 8 * hh;
+#pragma unroll
+    for (int kk = 0; kk < KT; ++kk) qraw[kk] = *reinterpret_cast<const u32x4*>(qr + 16 * kk);
+  }
+  const int L = p.t.cached(b);
   const TreeTiles tl(L, N, p.nspan, KEYS, KW);
   if (s >= tl.spans) return;  // the combine does not read this span
   const int steps = min(tl.per, (tl.all - s * KW * tl.per + KW - 1) / KW);
@@ -418,7 +404,7 @@ __global__ __launch_bounds__(64 * tree_waves<D>()) void tree_attn_rows_kernel(Tr
   const uint16_t* vc = p.vc + b * p.svc[0] + (int64_t)kvh * p.svc[1];
   const uint16_t* kn = p.k + b * p.sk[0] + (int64_t)kvh * p.sk[1];
   const uint16_t* vn = p.v + b * p.sv[0] + (int64_t)kvh * p.sv[1];
-  const uint64_t anc = tree_ancestors(p.t, b, lane);
+  const uint64_t anc = tree_ancestors(up, lane), above = shfl64(anc, node), seen = row < RN ? above : 0ull;
   const uint64_t padding = ~__ballot(anc != 0ull);
   WaveStager<uint16_t, D, 16> ks, vs;
   ks.init(p.skc[2], lane);
@@ -445,19 +431,9 @@ __global__ __launch_bounds__(64 * tree_waves<D>()) void tree_attn_rows_kernel(Tr
     }
   };
   stage(first, 0);
-
-  const int row = (rb * RW + rw) * 32 + l32, rc = min(row, RN - 1), node = rc % N;
-  const bool active = (rb * RW + rw) * 32 < RN;  // wave-uniform
-  const uint64_t up = shfl64(anc, node), seen = row < RN ? up : 0ull;
   V8 qop[KT];
-  {
-    const uint16_t* qr = p.q + b * p.sq[0] + (int64_t)(kvh * p.R + rc / N) * p.sq[1] + (int64_t)node * p.sq[2] + 8 * hh;
 #pragma unroll
-    for (int kk = 0; kk < KT; ++kk) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(qr + 16 * kk);
-      qop[kk] = __builtin_bit_cast(V8, seen ? x : zero4());
-    }
-  }
+  for (int kk = 0; kk < KT; ++kk) qop[kk] = __builtin_bit_cast(V8, seen ? qraw[kk] : zero4());
   f32x16 oacc[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) zero16(oacc[dt]);
