@@ -64,13 +64,14 @@ def attention_inputs(b, hq, hkv, d, n, cap, dtype, seed, sigma=1.0):
     return [q, k, v, r(b, hkv, cap, d), r(b, hkv, cap, d)]
 
 
-def check_attention(out, q, k, v, kc, vc, lengths, parents, name=""):
+def check_attention(out, q, k, v, kc, vc, lengths, parents, name="", steps=0):
+    """steps: fp32 additions of a long sum, beyond those that the 2^-16 covers."""
     d, h = q.shape[-1], half_step(out.dtype)
     got = np64(out)
     q, k, v, kc, vc = (np64(x) for x in (q, k, v, kc, vc))
     for i, (n, par) in enumerate(zip(lengths, parents)):
         ref, mag, top = orc.tree_attention(q[i], k[i], v[i], kc[i], vc[i], int(n), list(par), 1 / math.sqrt(d))
-        share = 2 * (d + 8) * 2.0 ** -24 * (top[..., None] + 1) + 2.0 ** -16
+        share = 2 * (d + 8) * 2.0 ** -24 * (top[..., None] + 1) + 2.0 ** -16 + steps * 2.0 ** -24
         bound = (h + share) * (mag + abs(ref)) + h * abs(ref) + 1e-30
         if out.dtype == FP16:
             bound = bound + 2.0 ** -25  # half a step among the subnormals
@@ -121,6 +122,48 @@ def test_tree_attention_matches_the_oracle(mta, case):
     check_attention(same, *cpu, [lengths[0]] * b, [par[0]] * b, "int length")
     one = mta.tree_attention(q, k, v, kc, vc, length[:1], parents[0], repeats=hq // hkv)
     check_attention(one, *cpu, [lengths[0]] * b, [par[0]] * b, "one length")
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("repeats,n", [(4, 16), (4, 27), (8, 21)], ids=["rows64", "rows108", "rows168"])
+def test_more_heads_than_the_card_takes_at_once(mta, repeats, n, d):
+    """132 KV heads of all sequences, so that a workgroup takes 64, 128 and 256 query rows on one key tile: lengths
+    about its tiles' ends, and padding and unseen cache rows that hold anything."""
+    b, hkv, cap, dtype = 33, 4, 300, FP16 if d == 64 else BF16
+    cpu = attention_inputs(b, hkv * repeats, hkv, d, n, cap, dtype, seed=n + d)
+    par = trees("padded", b, n, seed=d)
+    edges = [0, 1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 299, 300]
+    lengths = [edges[i % 16] for i in range(b)]
+    q, k, v, kc, vc = (x.to(DEV) for x in cpu)
+    parents, length = (torch.tensor(np.asarray(x), dtype=torch.int32, device=DEV) for x in (par, lengths))
+    out = mta.tree_attention(q, k, v, kc, vc, length, parents, repeats=repeats)
+    pick = list(range(16)) + [b - 1]
+    check_attention(out[pick], *(x[pick] for x in cpu), [lengths[i] for i in pick], par[pick])
+    assert torch.equal(out, mta.tree_attention(q, k, v, kc, vc, length, parents, repeats=repeats)), "the same call twice"
+    padding = torch.tensor([[u is None for u in orc.ancestors(list(p))] for p in par], device=DEV)
+    assert bool(padding.any()) and (out.transpose(1, 2)[padding] == 0).all()
+    for bad in (math.nan, -math.inf):
+        for x in (q, k, v):
+            x.transpose(1, 2)[padding] = bad
+        for i, m in enumerate(lengths):
+            kc[i, :, m:] = bad
+            vc[i, :, m:] = bad
+        assert torch.equal(mta.tree_attention(q, k, v, kc, vc, length, parents, repeats=repeats), out), bad
+
+
+@pytest.mark.parametrize("d,n,cap", [(128, 16, 8300), (128, 16, 65700), (128, 64, 131200),
+                                     (64, 64, 6300), (64, 64, 49300), (32, 64, 393300)])
+def test_many_rows_on_a_long_cache(mta, d, n, cap):
+    """64 heads of one KV head on caches so long that a workgroup takes 64, 128 and 256 rows, its keys shared out."""
+    g = torch.Generator(DEV).manual_seed(cap)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV).to(BF16)  # noqa: E731
+    q, k, v, kc, vc = r(1, 64, n, d), r(1, 1, n, d), r(1, 1, n, d), r(1, 1, cap, d), r(1, 1, cap, d)
+    par = trees("forest", 1, n, 6)
+    parents = torch.tensor(par, dtype=torch.int32, device=DEV)
+    for length in (cap - 33, cap):
+        out = mta.tree_attention(q, k, v, kc, vc, length, parents, repeats=64)
+        one = [0 if length == cap else 63]
+        check_attention(out[:, one], q[:, one], k, v, kc, vc, [length], par, steps=cap / 16)
 
 
 def test_one_node_is_decode_attention(mta):
