@@ -140,13 +140,15 @@ void launch_tree(const mt::TreeAttnParams& p, int rw, unsigned grid, hipStream_t
                        st, p);
 }
 
-// Nodes of a sequence whose rows are taken before the walk: as many as the card works on at a time.
-// A row of up to 16384 words leaves room for others on its CU, a longer one hardly.  Rows and walk, us:
-// 32 sequences of 16 nodes with a drafter, 16384 fp32 words, 4 rows a CU (all nodes) 21.0 + 10.5, 2 rows
-// 11.1 + 26.5, 1 row 9.0 + 32.7; 64 sequences of 64 nodes, 32001 16-bit words, 4 rows a CU 48.8 + 19.4, 2 rows
-// 25.4 + 19.3, 1 row 13.6 + 19.3.
+// Nodes of a sequence whose rows are taken before the walk, in rows a CU.  A drafter's tokens are mostly
+// accepted and its walks long, and each node that is taken on the way costs two rows one after the other; a walk
+// without a drafter's probabilities is short.  Rows and walk, us, at 1, 2 and 4 rows a CU; fp32:
+//   drafter, 32 sequences of 16 nodes, 16384 words:  6 + 25,  8 + 21, 15 + 10;  32001 words: 10 + 75, 20 + 51, 36 + 12
+//   drafter, 16 sequences of 64 nodes, 16384 words:  6 + 48,  8 + 50, 16 + 12;  32001 words: 10 + 39, 20 + 39, 37 + 16
+//   none, 16 sequences of 64 nodes, 16384 words:     6 + 12,  8 + 9,  16 + 9
+//   none, 64 sequences of 64 nodes, 32001 16-bit words: 9.5 + 15, 13 + 15, 22 + 15
 int verify_ahead(int64_t B, int N, int vocab, bool draft) {
-  const int64_t rows = (vocab <= 16384 ? 4 : 1) * (int64_t)device_cus();
+  const int64_t rows = (draft ? 4 : vocab <= 16384 ? 2 : 1) * (int64_t)device_cus();
   return (int)std::max<int64_t>(1, std::min<int64_t>(N, rows / (B * (draft ? 2 : 1))));
 }
 
@@ -163,15 +165,15 @@ void launch_verify(const mt::VerifyParams& p, hipStream_t st) {
   else hipLaunchKernelGGL((mt::verify_walk_kernel<DT, T, C, false>), walks, block, 0, st, p);
 }
 
-// A row in 32 registers a thread (at most 16 for a short vocabulary): 64 16-bit values or 32 fp32 ones.
-// More waves a row cost more than they bring (512 against 1024 threads for the rows above: 21.0 / 35.9 and
-// 49.8 / 50.7 us): what a wave does for itself, the ballots of the bound above all, is most of a row's time.
+// A row in 32 registers a thread, 64 for fp32 (a quarter for a short vocabulary): 64 values.  Twice the threads and
+// half the values take longer (rows and walk, 16384 fp32 words: 15.2 + 10.0 us against 17.8 + 10.0; 32001 fp32
+// words 10.7 + 15.7 against 12.7 + 19.1, 16-bit words 9.5 + 14.8 against 11.8 + 17.9): what a wave does for itself, the
+// ballots of the bound above all, is much of a row's time.
 template <int DT>
 void launch_verify_v(const mt::VerifyParams& p, hipStream_t st) {
-  constexpr bool wide = DT == kDtFP32;
   if (p.V <= 4096) launch_verify<DT, 256, 2>(p, st);
-  else if (p.V <= 16384) launch_verify<DT, wide ? 512 : 256, wide ? 4 : 8>(p, st);
-  else launch_verify<DT, wide ? 1024 : 512, wide ? 4 : 8>(p, st);
+  else if (p.V <= 16384) launch_verify<DT, 256, 8>(p, st);
+  else launch_verify<DT, 512, 8>(p, st);
 }
 
 int check_distill(int64_t ld, int64_t rows, int vocab, int entries, float temperature, int dtype) {

@@ -23,6 +23,11 @@
 // A walk visits a few nodes, but which is known only as it goes.  The rows of the
 // first `ahead` nodes of every sequence are taken before it, all at once: as many as
 // the card holds at a time.  A node past them is taken when the walk reaches it.
+//
+// Bound by latency: one row alone takes 7 to 8 us from its loads over the bound, the list and the ranks to
+// the sum, a node of the walk 1 to 3 us.  32 sequences of 16 nodes with a drafter, 16384 fp32 words:
+// 15.2 us for the 67 MB of 1024 rows (4.4 TB/s) and 10.1 for the walks; 64 sequences of 64 nodes without one,
+// 32001 bf16 words: 9.5 us for the 16 MB of 256 rows and 14.8 for the walks.
 #pragma once
 
 #include "sample_kernels.h"
@@ -78,6 +83,17 @@ struct RowLds {
   int count[T / 64];
   uint32_t kth;
 };
+
+// x of the wave's lanes up to this one, added
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, rows of 16 lanes
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
 
 // block-wide max or sum; barriers at both ends of buf's use
 template <int T, bool MAX>
@@ -183,8 +199,8 @@ __device__ __forceinline__ uint32_t kth_key(const Row<DT, T, C>& x, int k, float
 // The values that count are those >= t, t below the k-th largest and at least max - 110, where
 // an exponential is 0.  k <= T: every wave finds the ceil(k / waves)-th and the k-th
 // largest of its lanes' maxima, a ballot a bit; at least k values are >= the smallest
-// of the former and >= the largest of the latter.  About twice k random values pass; in
-// LDS, a value that fewer than k of them exceed is kept: ties of the k-th stay.  k > T:
+// of the former and >= the largest of the latter.  Two to four times k random values pass;
+// in LDS, a value that fewer than k of them exceed is kept: ties of the k-th stay.  k > T:
 // the k-th largest itself, bit by bit with block-wide counts.
 template <int DT, int T, int C>
 __device__ __forceinline__ RowTop row_top(const void* base, int64_t row, int V, int k, RowLds<T>& s) {
@@ -233,12 +249,7 @@ __device__ __forceinline__ RowTop row_top(const void* base, int64_t row, int V, 
   int mine = 0;
 #pragma unroll
   for (int w = 0; w < (C + 3) / 4; ++w) mine += __popc(in[w]);
-  int upto = mine;  // of the wave's threads up to this one
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(upto, o, 64);
-    if (lane >= o) upto += y;
-  }
+  const int upto = wave_scan(mine);
   if (lane == 63) s.count[wave] = upto;
   __syncthreads();
   int at = upto - mine, n = 0;
@@ -249,34 +260,42 @@ __device__ __forceinline__ RowTop row_top(const void* base, int64_t row, int V, 
     n += c;
   }
   if (n <= kVerifyList) {
+// the indexes from the registers; the values are loaded once more, in a thread of their own each: from
+    // the registers, which nothing can index, every one of them would be stored under a condition
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const uint32_t bits = in[c / 4] >> (8 * (min(C, 4) - 1 - c % 4)) & 255u;
-      if (!bits) continue;  // few threads have any
-      float v[8];
-      x.get(c, v);
-      const int word = Row<DT, T, C>::word(c, V);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (bits >> (7 - e) & 1u) {
-          s.key[at] = sample_key(fminf(v[e], __FLT_MAX__) + 0.f);
-          s.idx[at++] = word + e;
-        }
+    for (int w = 0; w < (C + 3) / 4; ++w) {
+      constexpr int kSlots = 8 * (C < 4 ? C : 4);
+      for (uint32_t bits = in[w]; bits; ++at) {
+        const int bit = 31 - __builtin_clz(bits), slot = kSlots - 1 - bit;
+        s.idx[at] = Row<DT, T, C>::word(4 * w + slot / 8, V) + slot % 8;
+        bits ^= 1u << bit;
+      }
     }
-    const int pad = n + tid;  // up to three zero keys complete the last group of four
-    if (tid < 3 && pad < kVerifyList) s.key[pad] = 0u;
+    __syncthreads();
+    for (int i = tid; i < n; i += T) s.key[i] = sample_key(load_logit<DT>(base, row + s.idx[i]));
+    const int pad = n + tid;  // zero keys complete the last group of 64
+    if (tid < 63 && pad < kVerifyList) s.key[pad] = 0u;
     __syncthreads();
     if (k < V && k <= T) {
-      for (int i = tid; i < n; i += T) {
-        const uint32_t own = s.key[i];
+      float least = INFINITY;  // of the values that fewer than k exceed; four threads count for one
+      for (int i = tid / 4; i - tid / 4 < n; i += T / 4) {
+        const uint32_t own = s.key[min(i, n - 1)];
         int larger = 0;
-        for (int c = 0; c < n; c += 4) {
-          const u32x4 q = *reinterpret_cast<const u32x4*>(&s.key[c]);
+        for (int c = 4 * (tid & 3); c < n; c += 64) {
+          u32x4 q[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) larger += q[e] > own ? 1 : 0;
+          for (int g = 0; g < 4; ++g) q[g] = *reinterpret_cast<const u32x4*>(&s.key[c + 16 * g]);
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) larger += q[g][e] > own ? 1 : 0;
         }
-        if (larger < k) atomicMin(&s.kth, own);
+        larger += __builtin_amdgcn_update_dpp(0, larger, 0xB1, 0xf, 0xf, false);  // the lanes of a quad
+        larger += __builtin_amdgcn_update_dpp(0, larger, 0x4E, 0xf, 0xf, false);
+        if (larger < k) least = fminf(least, sample_unkey(own));
       }
+      least = -wave_reduce<0, true>(-least);
+      if (lane == 0 && least < INFINITY) atomicMin(&s.kth, sample_key(least + 0.f));
       __syncthreads();
       r.kth = s.kth;
     }
@@ -366,7 +385,7 @@ __global__ __launch_bounds__(T) void verify_walk_kernel(VerifyParams p) {
     const int64_t xat = b * p.s[0][0] + here * p.s[0][1], yat = DRAFT ? b * p.s[1][0] + here * p.s[1][1] : 0;
     const bool ready = here < p.ahead;
     RowTop tp, tq{};
-    if (ready) {
+    if (__builtin_expect(ready, 1)) {
       tp = s.top[0][here];
       if constexpr (DRAFT) tq = s.top[1][here];
     } else {
