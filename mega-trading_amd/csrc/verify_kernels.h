@@ -242,7 +242,8 @@ __device__ __forceinline__ RowTop row_top(const void* base, int64_t row, int V, 
     return r;
   }
   r.kth = sample_key(r.max - 110.f + 0.f);
-  if (k < V) r.kth = max(r.kth, k <= T ? max(t1, t2) : kth_key(x, k, s.buf));
+  // +inf counts as the highest float, whose words it must not push out
+  if (k < V) r.kth = max(r.kth, min(k <= T ? max(t1, t2) : kth_key(x, k, s.buf), sample_key(__FLT_MAX__)));
   const float t = sample_unkey(r.kth);
   uint32_t in[(C + 3) / 4] = {};  // the slots that count, 32 a word, the first in the highest bit
   x.each([&](float v, int j) { in[j / 32] += in[j / 32] + (v >= t ? 1u : 0u); });
@@ -311,7 +312,7 @@ __device__ __forceinline__ RowTop row_top(const void* base, int64_t row, int V, 
     Row<DT, T, C> again;  // not kept in registers until here
     asm volatile("" : "+s"(base));
     again.load(base, row, V);
-    r.kth = max(r.kth, kth_key(again, k, s.buf));
+    r.kth = max(r.kth, min(kth_key(again, k, s.buf), sample_key(__FLT_MAX__)));
   }
   float sum = 0.f;
   for (int i = tid; i < V; i += T) {

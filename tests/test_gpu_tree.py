@@ -454,6 +454,21 @@ def test_verify_ties_masks_and_odd_tokens(mta, drafted):
     check_verify(mta, s, "zeros")
 
 
+@pytest.mark.parametrize("vocab", [40, 5000, 20000])
+def test_verify_counts_infinity_as_the_highest_number(mta, vocab):
+    # +inf and the largest float are one logit: with k = 1 both words stay, and the noise decides
+    for k, at in ((1, 4), (1, vocab - 1), (2, vocab - 1)):
+        s = verify_inputs(3, 2, vocab, k, F32, False, vocab + k)
+        s["logits"][:, :, 3] = math.inf
+        s["logits"][:, :, at] = torch.finfo(F32).max
+        s["tokens"][:, 1] = at
+        s["uniform"][:] = torch.tensor([[0.0, 0.25], [0.0, 0.75], [0.0, 0.75]])
+        s["noise"][:, 3] = 2.0
+        s["noise"][1, 3], s["noise"][0, at], s["noise"][2, at] = 3.0, 1.0, 4.0
+        path, count, token = check_verify(mta, s, f"k {k} at {at}")
+        assert count.tolist() == [2, 1, 1] and token.flatten().tolist() == [at, 3, 3]
+
+
 def test_verify_layouts(mta):
     s = verify_inputs(4, 6, 515, 16, BF16, True, 7)
     dev = {a: x.to(DEV) if torch.is_tensor(x) else x for a, x in s.items()}
