@@ -37,6 +37,7 @@ MAX_DECODE_REPEATS = 8
 
 # nodes of one drafted tree (a node's ancestors are one 64-bit word)
 MAX_TREE_NODES = 64
+_MOST_ROWS = 0x7FFFFF00  # of a cache or a RoPE table: the tree kernels count them in 32 bits
 
 # head sizes the kernels are built for; any other head_dim up to MAX_HEAD_DIM is
 # zero-padded to the next one (the reference's forward takes any D, rounding its
@@ -358,6 +359,7 @@ def tree_commit(keys, values, path: torch.Tensor, count: torch.Tensor, length, k
     ``keys`` / ``values``: one [B, Hkv, N, D] tensor per layer, as that layer's
     ``tree_attention`` took them; ``key_caches`` / ``value_caches``: one
     [B, Hkv, capacity, D] tensor per layer, written in place (unit last stride).
+    The nodes' tensors and the caches must not overlap, and no two nodes' tensors share a cache.
     ``path`` [B, N] and ``count`` [B] int32 as ``ops.topk_verify`` returns them,
     ``length`` as for ``tree_attention``: the cached tokens before this call, which
     are ``length + count`` after it.  Nodes outside the tree and positions at or
@@ -390,8 +392,8 @@ def _check_tree_rope(query, key, cos, sin, length_dev, length, parents) -> None:
         if tab.device != query.device:
             raise RuntimeError("RoPE tables must be on the device of query")
     rows = min(cos.numel(), sin.numel()) // (d // 2)
-    if rows < 1:
-        raise ValueError("the RoPE tables must have rows")
+    if not 1 <= rows <= _MOST_ROWS:
+        raise ValueError(f"the RoPE tables must have rows, fewer than 2^31 (got {rows})")
     _check_tree(parents, length_dev, length, b, n, rows - 1, query.device)
 
 
@@ -420,6 +422,8 @@ def _check_tree_commit(keys, values, path, count, length_dev, length, key_caches
             raise ValueError("the caches must share one shape")
         if kc.stride(-1) != 1 or vc.stride(-1) != 1:
             raise ValueError("the caches must have a unit last-dim stride")
+        if any(t.shape[i] > 1 and t.stride(i) == 0 for t in (kc, vc) for i in range(3)):
+            raise ValueError("the caches must not be expanded")
     b, _, n, _ = first.shape
     for name, t, shape in (("path", path, (b, n)), ("count", count, (b,))):
         if t.dtype != torch.int32 or tuple(t.shape) != shape:
@@ -452,6 +456,8 @@ def _check_caches(key_cache, value_cache, key) -> None:
         raise ValueError("key and value caches must have the same shape [batch, heads, capacity, head_dim]")
     if key_cache.shape[:2] != key.shape[:2] or key_cache.shape[3] != key.shape[3]:
         raise ValueError("the caches must have the batch, heads and head_dim of the nodes' keys")
+    if key_cache.shape[2] > _MOST_ROWS:
+        raise ValueError(f"a capacity of {key_cache.shape[2]} is too large")
     for t in (key_cache, value_cache):
         if t.dtype != key.dtype or t.device != key.device:
             raise RuntimeError("the caches must have the dtype and device of the nodes' keys")

@@ -312,6 +312,7 @@ Tree tree(const std::optional<at::Tensor>& parents, const std::optional<at::Tens
 // The checks of the calls, here for the GPU's tensors and in Python (attention.py, ops.py) for traced ones: in
 // Python they cost as much as the rest of a small call (5 nodes on a cache 11.4 -> 7.2 us a call, the write
 // into 8 layers' caches 35.2 -> 10.5).
+constexpr int64_t kMostRows = 0x7fffff00;  // of a cache or a table, and nodes in all: the kernels count them in 32 bits
 void check_nodes(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, bool fp32) {
   const at::ScalarType t = q.scalar_type();
   TORCH_CHECK(t == at::kBFloat16 || t == at::kHalf || (fp32 && t == at::kFloat), "unsupported dtype ", t);
@@ -324,6 +325,7 @@ void check_nodes(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, 
                     "query heads must be a positive multiple of the key/value heads");
   TORCH_CHECK_VALUE(q.size(0) > 0 && q.size(2) >= 1 && q.size(2) <= 64, "need a batch and 1 to 64 nodes (got ", q.size(0),
                     ", ", q.size(2), ")");
+  TORCH_CHECK_VALUE(q.size(0) <= kMostRows / (q.size(1) * q.size(2)), "too many nodes");
   for (const at::Tensor* x : {&k, &v})
     TORCH_CHECK(x->scalar_type() == t && x->device() == q.device(), "query, key and value must share one dtype and device");
 }
@@ -332,6 +334,7 @@ void check_caches(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& 
                     "key and value caches must have the same shape [batch, heads, capacity, head_dim]");
   TORCH_CHECK_VALUE(kc.size(0) == key.size(0) && kc.size(1) == key.size(1) && kc.size(3) == key.size(3),
                     "the caches must have the batch, heads and head_dim of the nodes' keys");
+  TORCH_CHECK_VALUE(kc.size(2) <= kMostRows, "a capacity of ", kc.size(2), " is too large");
   for (const at::Tensor* x : {&kc, &vc})
     TORCH_CHECK(x->scalar_type() == key.scalar_type() && x->device() == key.device(),
                 "the caches must have the dtype and device of the nodes' keys");
@@ -367,6 +370,16 @@ void check_parents(const at::Tensor& t, int64_t b, int64_t n, at::Device device)
 // in place where the kernels can read it, else a copy
 at::Tensor rows16(const at::Tensor& t) { return kernel_ready(t) ? t : flat(t); }
 
+// the bytes from a tensor's first value to its last
+using Span = std::pair<uintptr_t, uintptr_t>;
+Span span(const at::Tensor& t) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
+  if (t.numel() == 0) return {at, at};
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  return {at, at + (last + 1) * t.element_size()};
+}
+
 std::tuple<at::Tensor, at::Tensor> tree_rope(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& cos,
                                              const at::Tensor& sin, const std::optional<at::Tensor>& length_dev,
                                              int64_t length, const at::Tensor& parents) {
@@ -379,7 +392,7 @@ std::tuple<at::Tensor, at::Tensor> tree_rope(const at::Tensor& q_in, const at::T
     TORCH_CHECK(t->device() == q_in.device(), "RoPE tables must be on the device of query");
   }
   const int64_t rows = std::min(cos.numel(), sin.numel()) / half;
-  TORCH_CHECK_VALUE(rows > 0, "the RoPE tables must have rows");
+  TORCH_CHECK_VALUE(rows > 0 && rows <= kMostRows, "the RoPE tables must have rows, fewer than 2^31 (got ", rows, ")");
   check_parents(parents, q_in.size(0), q_in.size(2), q_in.device());
   check_length(length_dev, length, q_in.size(0), rows - 1, q_in.device());
   const c10::DeviceGuard guard(q_in.device());
@@ -448,7 +461,23 @@ void tree_commit(at::TensorList keys, at::TensorList values, const at::Tensor& p
     TORCH_CHECK_VALUE(key_caches[l].sizes() == key_caches[0].sizes(), "the caches must share one shape");
     TORCH_CHECK_VALUE(key_caches[l].stride(3) == 1 && value_caches[l].stride(3) == 1,
                       "the caches must have a unit last-dim stride");
+    for (const at::Tensor* x : {&key_caches[l], &value_caches[l]})
+      for (int i = 0; i < 3; ++i)
+        TORCH_CHECK_VALUE(x->size(i) < 2 || x->stride(i) != 0, "the caches must not be expanded");
   }
+  // nodes that lie in a cache could be overwritten before they are read
+  std::vector<Span> to, from;
+  for (const at::TensorList& l : {key_caches, value_caches})
+    for (const at::Tensor& x : l) to.push_back(span(x));
+  for (const at::TensorList& l : {keys, values})
+    for (const at::Tensor& x : l) from.push_back(span(x));
+  for (const Span& x : from)
+    for (const Span& y : to)
+      TORCH_CHECK_VALUE(x.first >= y.second || y.first >= x.second, "keys and values must not overlap the caches");
+  for (size_t i = 0; i < to.size(); ++i)
+    for (size_t j = 0; j < i; ++j)
+      TORCH_CHECK_VALUE(to[i].first != to[j].first || to[i].first == to[i].second || from[i].first == from[j].first,
+                        "one cache must not take the nodes of two");
   check_ints("path", path_in, at::kInt, {keys[0].size(0), keys[0].size(2)}, keys[0].device());
   check_ints("count", count_in, at::kInt, {keys[0].size(0)}, keys[0].device());
   check_length(length_dev, length, keys[0].size(0), key_caches[0].size(2), keys[0].device());
@@ -501,6 +530,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> topk_verify(const at::Tensor& log
     const int64_t b = logits.size(0), n = logits.size(1), v = logits.size(2);
     const at::Device dev = logits.device();
     TORCH_CHECK_VALUE(n >= 1 && n <= 64, "need 1 to 64 nodes (got ", n, ")");
+    TORCH_CHECK_VALUE(b <= kMostRows / 128, "too many sequences (", b, ")");
     TORCH_CHECK_VALUE(1 <= k && k <= v && v <= 32768, "need 1 <= k <= vocab <= 32768 (k=", k, ", vocab=", v, ")");
     check_ints("tokens", tokens_in, at::kLong, {b, n}, dev);
     check_parents(parents, b, n, dev);
@@ -544,7 +574,7 @@ int64_t row_stride(const at::Tensor& r) { return r.size(0) > 1 ? r.stride(0) : r
 void check_distill(const at::Tensor& x, const at::Tensor& y, const at::Tensor& i) {
   check_float("logits", x);
   check_float("teacher_logits", y);
-  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "logits must have shape [..., vocab]");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= kMostRows, "logits must have shape [..., vocab]");
   TORCH_CHECK_VALUE(y.dim() == x.dim() && y.sizes().slice(0, y.dim() - 1) == x.sizes().slice(0, x.dim() - 1),
                     "teacher_logits must have shape [..., entries] with the rows of logits");
   TORCH_CHECK_VALUE(i.sizes() == y.sizes(), "teacher_indices must have the shape of teacher_logits");

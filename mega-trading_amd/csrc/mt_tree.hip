@@ -52,7 +52,8 @@ int check_tree(int B, int N, const int* parents, int64_t parents_stride, const i
                int length, int capacity) {
   if (B < 1 || N < 1 || N > mt::kTreeNodes)
     return fail(MT_E_SHAPE, "B must be >= 1 and the nodes in [1, %d] (got %d, %d)", mt::kTreeNodes, B, N);
-  if (capacity < 0) return fail(MT_E_SHAPE, "capacity %d is negative", capacity);
+  if (capacity < 0 || capacity > 0x7fffff00)  // tiles past the end are counted in 32 bits
+    return fail(MT_E_SHAPE, "capacity %d is negative or too large", capacity);
   if (!parents) return fail(MT_E_NULL, "parents is NULL");
   if (parents_stride != 0 && parents_stride < N)
     return fail(MT_E_STRIDE, "parents stride %lld must be 0 or at least the nodes", (long long)parents_stride);

@@ -192,6 +192,63 @@ __device__ __forceinline__ void tree_merge(const TreeAttnParams& p, int pair, in
   }
 }
 
+// Whether one of the 8 values is infinite or NaN.
+template <class E>
+__device__ __forceinline__ bool not_finite(u32x4 x) {
+  constexpr uint32_t M = std::is_same<E, BF16>::value ? 0x7f80u : 0x7c00u;
+  bool r = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r |= (x[i] & M) == M || (x[i] >> 16 & M) == M;
+  return r;
+}
+
+// The rows of a tile of nodes, one row after the other over NC lanes each (chunk x, taken or not): which of them
+// hold a value that is no number, bit by bit; and whether this lane's row does.
+template <class E, int NC>
+__device__ __forceinline__ uint32_t odd_rows(u32x4 x, bool taken, int lane, bool& mine) {
+  const uint64_t bad = __ballot(taken && not_finite<E>(x));
+  constexpr uint64_t ROW = (1ull << NC) - 1;
+  mine = (bad >> (lane / NC * NC) & ROW) != 0;
+  uint32_t rows = 0u;
+  if (bad)
+#pragma unroll
+    for (int r = 0; r < 64 / NC; ++r) rows |= (bad >> (r * NC) & ROW) ? 1u << r : 0u;
+  return rows;
+}
+
+// A node's values that are no numbers reach its descendants alone: in the tiles, where every row multiplies
+// them, 0 stands for all of its values, and the rows that see it (query row `row`) add them here, by the formula.
+template <class E, int D>
+__device__ __forceinline__ void tree_add_odd(const TreeAttnParams& p, uint64_t odd, uint64_t seen, int b, int kvh, int row,
+                                             int hh, float m, f32x16 (&o)[D / 32]) {
+  const int rc = min(row, p.R * p.t.N - 1);
+  const uint16_t* q = p.q + b * p.sq[0] + (int64_t)(kvh * p.R + rc / p.t.N) * p.sq[1] + (int64_t)(rc % p.t.N) * p.sq[2] + 8 * hh;
+  const uint16_t* k = p.k + b * p.sk[0] + (int64_t)kvh * p.sk[1] + 8 * hh;
+  const uint16_t* v = p.v + b * p.sv[0] + (int64_t)kvh * p.sv[1] + 4 * hh;
+  for (; odd; odd &= odd - 1) {
+    const int n = __builtin_ctzll(odd);
+    float s = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(q + 16 * kk), y = *reinterpret_cast<const u32x4*>(k + n * p.sk[2] + 16 * kk);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = E::dot2(x[e], y[e], s);
+    }
+    s = sum_with_partner(s);
+    if (!(seen >> n & 1)) continue;
+    const float w = exp2_fast(__builtin_fmaf(s, p.scale_log2, -m));
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(v + n * p.sv[2] + 32 * dt + 8 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o[dt][4 * i + e] = __builtin_fmaf(w, E::to_f((uint16_t)(x[e / 2] >> (16 * (e % 2)))), o[dt][4 * i + e]);
+      }
+  }
+}
+
 template <int D>
 constexpr int tree_few_waves() { return D == 128 ? 4 : 8; }  // what the tiles leave room for: one workgroup a CU
 
@@ -256,6 +313,7 @@ __global__ __launch_bounds__(64 * tree_few_waves<D>()) void tree_attn_kernel(Tre
   const int rbase = TL::row_base(lane);
   const TrBase tbase = TL::tr_base(lane);
   const float c2 = p.scale_log2;
+  uint64_t odd = 0ull;  // nodes with a value that is no number
 
   if (t0 < t1) stage(t0, 0);
   if (t0 + 1 < t1) stage(t0 + 1, 1);
@@ -268,8 +326,13 @@ __global__ __launch_bounds__(64 * tree_few_waves<D>()) void tree_attn_kernel(Tre
     if (n0 >= 0) {
       // values of padding may be anything, and 0 times it must be 0
 #pragma unroll
-      for (int i = lane; i < kTreeKeys * TL::NC; i += 64)
-        if (padding >> (n0 + i / TL::NC) & 1) *reinterpret_cast<u32x4*>(vl + i * 16) = zero4();
+      for (int i = 0; i < TL::NC / 2; ++i) {
+        char* at = vl + (i * 64 + lane) * 16;
+        const bool pad = padding >> (n0 + (i * 64 + lane) / TL::NC) & 1;
+        bool mine;
+        odd |= (uint64_t)odd_rows<E, TL::NC>(*reinterpret_cast<const u32x4*>(at), !pad, lane, mine) << (n0 + i * (64 / TL::NC));
+        if (pad || mine) *reinterpret_cast<u32x4*>(at) = zero4();
+      }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -334,6 +397,7 @@ __global__ __launch_bounds__(64 * tree_few_waves<D>()) void tree_attn_kernel(Tre
     }
   }
   reads_done();
+  if (odd) tree_add_odd<E, D>(p, odd, seen, b, kvh, row, hh, mrun, oacc);
 
   // the wave's o, 16-byte chunk c of row r at slot c ^ (r mod C4)
   float* ow = reinterpret_cast<float*>(smem[wave]);
@@ -378,6 +442,7 @@ __global__ __launch_bounds__(64 * tree_waves<D>()) void tree_attn_rows_kernel(Tr
   constexpr bool AHEAD = D == 128;  // a quarter's scores beside the last one's softmax; else other waves' are
   __shared__ __attribute__((aligned(1024))) char smem[2][KW][2][TILE];  // then the waves' o [32][D] fp32
   __shared__ float wm[W][32], wl[W][32];
+  __shared__ uint32_t odd_lds[kTreeNodes / 16];  // nodes with a value that is no number, 16 a word
   static_assert(sizeof(smem) == W * 32 * D * 4, "the waves' o fill the tiles");
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kw = wave / RW, rw = wave % RW;
@@ -419,15 +484,19 @@ __global__ __launch_bounds__(64 * tree_waves<D>()) void tree_attn_rows_kernel(Tr
     } else {
       // the tree's, through registers: what padding holds is replaced by zeros, since 0 times it must be 0
       const int n0 = (t - tl.prefix) * KEYS + rw * 16;
+      uint32_t odd = 0u;
 #pragma unroll
       for (int i = 0; i < TL::NC / 4; ++i) {
         const int f = i * 64 + lane, row = f / TL::NC, chunk = (f % TL::NC) ^ TL::swz(row), n = n0 + row;
         const bool in = n < N && !(padding >> (n & 63) & 1);
         const u32x4 a = *reinterpret_cast<const u32x4*>(kn + (int64_t)min(n, N - 1) * p.sk[2] + chunk * 8);
         const u32x4 c = *reinterpret_cast<const u32x4*>(vn + (int64_t)min(n, N - 1) * p.sv[2] + chunk * 8);
+        bool mine;
+        odd |= odd_rows<E, TL::NC>(c, in, lane, mine) << (i * (64 / TL::NC));
         *reinterpret_cast<u32x4*>(kl + f * 16) = in ? a : zero4();
-        *reinterpret_cast<u32x4*>(vl + f * 16) = in ? c : zero4();
+        *reinterpret_cast<u32x4*>(vl + f * 16) = in && !mine ? c : zero4();
       }
+      if (n0 < kTreeNodes && lane == 0) odd_lds[n0 / 16] = odd;
     }
   };
   stage(first, 0);
@@ -441,6 +510,7 @@ __global__ __launch_bounds__(64 * tree_waves<D>()) void tree_attn_rows_kernel(Tr
   const int rbase = TL::row_base(lane);
   const TrBase tbase = TL::tr_base(lane);
   const float c2 = p.scale_log2;
+  uint64_t nodes = 0ull;  // of the group's tiles
 
   for (int i = 0; i < steps; ++i) {
     const int t = first + KW * i, buf = i & 1;
@@ -451,6 +521,7 @@ __global__ __launch_bounds__(64 * tree_waves<D>()) void tree_attn_rows_kernel(Tr
     const char *kl = smem[buf][kw][0], *vl = smem[buf][kw][1];
     const int n0 = (t - tl.prefix) * KEYS;  // the tile's first node, from 0 on
     const bool mask = n0 >= 0 || (t + 1) * KEYS > L;
+    if (n0 >= 0 && n0 < kTreeNodes) nodes |= (KEYS < 64 ? (1ull << (KEYS % 64)) - 1 : ~0ull) << n0;
     f32x16 st[AHEAD ? 2 : 1];
     auto scores = [&](int h, f32x16& x) {
 #pragma unroll
@@ -514,6 +585,13 @@ __global__ __launch_bounds__(64 * tree_waves<D>()) void tree_attn_rows_kernel(Tr
     }
   }
   __syncthreads();
+  if (nodes) {
+    uint64_t odd = 0ull;
+#pragma unroll
+    for (int i = 0; i < kTreeNodes / 16; ++i) odd |= (uint64_t)odd_lds[i] << (16 * i);
+    odd &= nodes;
+    if (odd) tree_add_odd<E, D>(p, odd, seen, b, kvh, row, hh, mrun, oacc);
+  }
 
   float* ow = reinterpret_cast<float*>(&smem[0][0][0][0]) + wave * 32 * D;
   {

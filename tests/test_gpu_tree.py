@@ -212,6 +212,42 @@ def test_what_is_not_seen_may_hold_anything(mta):
         assert torch.equal(got, out), bad
 
 
+@pytest.mark.parametrize("b,hkv,repeats,n,d,dtype", [
+    (3, 2, 4, 40, 64, BF16), (2, 1, 2, 64, 128, FP16), (2, 2, 1, 33, 32, BF16),
+    (33, 4, 4, 16, 64, BF16), (33, 4, 4, 27, 128, FP16), (33, 4, 8, 21, 64, FP16), (33, 4, 8, 21, 32, BF16)])
+def test_values_that_are_no_numbers_reach_descendants_alone(mta, b, hkv, repeats, n, d, dtype):
+    cap, length = 70, 45
+    cpu = attention_inputs(b, hkv * repeats, hkv, d, n, cap, dtype, seed=n)
+    par = trees("forest", b, n, 12)
+    dev = [x.to(DEV) for x in cpu]
+    parents = torch.tensor(par, dtype=torch.int32, device=DEV)
+    clean = mta.tree_attention(*dev, length, parents, repeats=repeats)
+    bad = [1, n // 2, n - 1]
+    for x in (cpu[2], dev[2]):
+        x[:, :, bad[0], 0] = math.inf
+        x[:, 0, bad[1], d - 1] = math.nan
+        x[:, :, bad[2], d // 2] = -math.inf
+    out = mta.tree_attention(*dev, length, parents, repeats=repeats)
+    seen = torch.tensor([[[m in up for m in bad] for up in orc.ancestors(list(q))] for q in par])  # [B, N, 3]
+    same = ~seen.any(-1)
+    assert bool(same.any()) and bool(seen.any())
+    assert torch.equal(out.transpose(1, 2).cpu()[same], clean.transpose(1, 2).cpu()[same])
+    h = half_step(dtype)
+    for i in (0, b - 1):
+        with np.errstate(invalid="ignore"):
+            ref, mag, top = orc.tree_attention(*(np64(x[i]) for x in cpu), length, list(par[i]), 1 / math.sqrt(d))
+        got, fine = np64(out[i]), np.isfinite(ref)
+        assert (fine == np.isfinite(got)).all() and (np.isnan(ref) == np.isnan(got)).all()
+        assert (np.sign(ref) == np.sign(got))[np.isinf(ref)].all()
+        share = 2 * (d + 8) * 2.0 ** -24 * (top[..., None] + 1) + 2.0 ** -16
+        bound = (h + share) * (np.where(fine, mag, 0) + abs(ref)) + h * abs(ref) + 2.0 ** -25
+        assert (abs(got[fine] - ref[fine]) <= bound[fine]).all()
+    for x in dev[:2]:  # and the same of queries and keys
+        x[:, :, bad] = math.nan
+    out = mta.tree_attention(*dev, length, parents, repeats=repeats)
+    assert torch.equal(out.transpose(1, 2).cpu()[same], clean.transpose(1, 2).cpu()[same])
+
+
 def test_layouts_streams_and_clamped_lengths(mta):
     b, hq, hkv, d, n, cap = 2, 8, 2, 64, 12, 96
     cpu = attention_inputs(b, hq, hkv, d, n, cap, FP16, seed=4)
@@ -369,6 +405,24 @@ def test_tree_commit_writes_the_accepted_rows_alone(mta, layers, d, dtype, layou
     # counts past the nodes stop at them; an int length
     mta.tree_commit(*nodes, path.to(DEV), torch.full((b,), 1000, dtype=torch.int32, device=DEV), 4, *caches)
     assert torch.equal(caches[0][0][1, :, 4:13], nodes[0][0][1])
+
+
+def test_tree_commit_refuses_shared_memory(mta):
+    """Nodes that lie in a cache, and a cache that two layers would write; what only lies in one allocation is written."""
+    g = gen(3)
+    both = torch.randn(4, 2, 2, 40, 64, generator=g).to(BF16).to(DEV)  # two layers' key and value caches
+    k, v = (torch.randn(2, 2, 5, 64, generator=g).to(BF16).to(DEV) for _ in range(2))
+    path = torch.tensor([[0, 1, 3, -1, -1]] * 2, dtype=torch.int32, device=DEV)
+    count = torch.full((2,), 3, dtype=torch.int32, device=DEV)
+    before = both.clone()
+    for keys, caches in (([both[0][:, :, 10:15]], [both[0]]), ([both[2][:, :, 10:15]], [both[0]]), ([k, v], [both[0], both[0]])):
+        with pytest.raises(ValueError, match="overlap|take the nodes of two"):
+            mta.tree_commit(keys, [v] * len(keys), path, count, 10, caches, [both[2], both[3]][:len(keys)])
+    assert torch.equal(both, before)
+    mta.tree_commit([k, k], [v, v], path, count, 10, [both[0], both[1]], [both[2], both[3]])
+    for i, x in enumerate((k, k, v, v)):
+        assert torch.equal(both[i][:, :, 10:13], x[:, :, [0, 1, 3]])
+        assert torch.equal(both[i][:, :, 13:], before[i][:, :, 13:]) and torch.equal(both[i][:, :, :10], before[i][:, :, :10])
 
 
 # ---------------------------------------------------------------------------

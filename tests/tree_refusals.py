@@ -36,6 +36,7 @@ def tree_attention(mta):
         (ValueError, "parents must be int32", lambda: mta.tree_attention(*args, 7, _new(4, dtype=torch.int32), repeats=2)),
         (ValueError, "agree on batch", lambda: mta.tree_attention(args[0], *_nodes(n=6)[1:3], *args[3:], 7, par, repeats=2)),
         (ValueError, "caches must have the batch", lambda: mta.tree_attention(*args[:3], *_nodes(b=3)[3:], 7, par, repeats=2)),
+        (ValueError, "too large", lambda: mta.tree_attention(*args[:3], *[t[:, :, :1].expand(2, 2, 1 << 33, 64) for t in args[3:]], 7, par, repeats=2)),
         (RuntimeError, "caches must have the dtype", lambda: mta.tree_attention(*args[:3], *_nodes(dtype=torch.float16)[3:], 7, par, repeats=2)),
     )
 
@@ -49,6 +50,8 @@ def tree_rope_and_commit(mta):
         (ValueError, "head_dim/2", lambda: mta.tree_rope(q, k, cs[..., :31], cs, 3, par)),
         (ValueError, "multiple of 8", lambda: mta.tree_rope(_new(2, 4, 5, 20), _new(2, 2, 5, 20), cs, cs, 3, par)),
         (ValueError, "must have rows", lambda: mta.tree_rope(q, k, cs[:, :, :0], cs, 0, par)),
+        (ValueError, "must have rows", lambda: mta.tree_rope(q, k, *[cs[:, :, :1].expand(1, 1, 1 << 32, 32)] * 2, 0, par)),
+        (ValueError, "expanded", lambda: mta.tree_commit([k], [v], path, count, 3, [kc[:1].expand(2, -1, -1, -1)], [vc])),
         (ValueError, "one tensor per layer", lambda: mta.tree_commit([], [], path, count, 3, [], [])),
         (ValueError, "one tensor per layer", lambda: mta.tree_commit([k, k], [v], path, count, 3, [kc], [vc])),
         (ValueError, "share one shape", lambda: mta.tree_commit([k], [v[:, :, :4]], path, count, 3, [kc], [vc])),
