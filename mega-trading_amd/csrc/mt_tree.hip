@@ -132,7 +132,7 @@ void launch_tree(const mt::TreeAttnParams& p, int rw, unsigned grid, hipStream_t
   else hipLaunchKernelGGL((mt::tree_attn_rows_kernel<E, D, 8>), dim3(grid), many, 0, st, p);
   if (p.nspan == 1) return;
   // up to 8 spans come in one batch of loads, and threads that share a row would only add their meeting
-  // (2 spans, 49152 rows of 128: 6.8 / 17.5 us; 118 spans, 512 rows of 64: 10.3 / 4.5)
+  // (2 spans, 12288 rows of 128: 6.8 / 17.5 us; 118 spans, 512 rows of 64: 10.3 / 4.5)
   const int64_t n = (int64_t)p.B * p.Hkv * p.R * p.t.N, few_rows = 256 / (D / 4), many_rows = few_rows / 8;
   if (p.nspan <= 8)
     hipLaunchKernelGGL((mt::tree_combine_kernel<E, D, 1>), dim3((unsigned)((n + few_rows - 1) / few_rows)), dim3(256), 0, st, p);
