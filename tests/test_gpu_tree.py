@@ -474,6 +474,21 @@ def test_topk_verify_matches_the_oracle(mta, b, n, vocab, k, dtype, kind, drafte
         check_verify(mta, verify_inputs(b, n, vocab, k, dtype, drafted, seed, kind), f"seed {seed}")
 
 
+@pytest.mark.parametrize("drafted", [True, False])
+@pytest.mark.parametrize("b,n,vocab,k,dtype,kind", [
+    (40, 40, 300, 16, F32, "chain"),    # walks past the rows that are taken ahead
+    (300, 9, 700, 4, BF16, "bush"),     # more sequences than the card takes at once
+    (64, 24, 17001, 20, FP16, "bush"),
+    (2, 6, 9000, 256, F32, "bush"),     # k at a workgroup's threads and past them, for each of its sizes
+    (2, 6, 9000, 257, F32, "bush"),
+    (2, 6, 20001, 512, F32, "bush"),
+    (2, 6, 20001, 513, BF16, "bush"),
+    (2, 6, 32768, 32768, F32, "bush"),
+])
+def test_topk_verify_past_the_card(mta, b, n, vocab, k, dtype, kind, drafted):
+    check_verify(mta, verify_inputs(b, n, vocab, k, dtype, drafted, 5, kind))
+
+
 def test_one_node_is_topk_sample(mta):
     for vocab, k in ((16384, 16), (1385, 50), (700, 700)):
         g = torch.Generator(device=DEV).manual_seed(vocab)
