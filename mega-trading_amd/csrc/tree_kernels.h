@@ -442,6 +442,8 @@ __global__ __launch_bounds__(64 * tree_few_waves<D>()) void tree_attn_kernel(Tre
 // LDS feeds up to 32 RW rows; W / RW key groups, 16 W keys a step in all.  Two buffers; every wave copies 16 rows
 // of its group's next tile while it works on the present one, and one barrier a step orders both.
 // Two waves a SIMD (four at D <= 64) let one's softmax run beside the other's products.
+// (D = 64, 64 KV heads of 256 rows on 10000 keys: 16 waves on tiles of 16 RW keys 61.6 us, 8 on tiles of
+// 32 RW keys 76.3; 8 of 512 rows on 15000 keys, join included: 34.4 and 37.6.)
 template <int D>
 constexpr int tree_waves() { return D == 128 ? 8 : 16; }  // what the tiles leave room for: one workgroup a CU
 
