@@ -26,8 +26,11 @@
 //
 // Bound by latency: one row alone takes 7 to 8 us from its loads over the bound, the list and the ranks to
 // the sum, a node of the walk 1 to 3 us.  32 sequences of 16 nodes with a drafter, 16384 fp32 words:
-// 15.2 us for the 67 MB of 1024 rows (4.4 TB/s) and 10.1 for the walks; 64 sequences of 64 nodes without one,
-// 32001 bf16 words: 9.5 us for the 16 MB of 256 rows and 14.8 for the walks.
+// 15.5 us for the 67 MB of 1024 rows (4.3 TB/s) and 10.0 for the walks; 64 sequences of 64 nodes without one,
+// 32001 bf16 words: 9.4 us for the 16 MB of 256 rows and 13.8 for the walks.  Without a list the walk goes over
+// whole rows: every word kept, 21 sequences of 46 nodes without a drafter, 21338 words: 9.9 and 32 us (a
+// rejected word's weight is subtracted; passes over the row instead took 111); 16 of 32 nodes with one, 32000 words:
+// 27 and 104; k = 2000 there: 78 (the k-th largest by bits) and 145.
 #pragma once
 
 #include "sample_kernels.h"
@@ -63,9 +66,10 @@ struct VerifyParams {
 constexpr int kVerifyList = 1024;  // values of a list
 
 // A logit as the operator counts it: finite, and no negative zero (its key is another).
+__device__ __forceinline__ float as_logit(float x) { return fminf(fmaxf(x, -__FLT_MAX__), __FLT_MAX__) + 0.f; }
 template <int DT>
 __device__ __forceinline__ float load_logit(const void* base, int64_t i) {
-  return fminf(fmaxf(ops::IO<DT>::load1(base, i), -__FLT_MAX__), __FLT_MAX__) + 0.f;
+  return as_logit(ops::IO<DT>::load1(base, i));
 }
 
 // A node's parent, or -2 for padding: only earlier nodes have children.
@@ -180,15 +184,19 @@ struct Row {
   }
 };
 
-// The key of the k-th largest value: the largest t with count(key >= t) >= k.
+// The key of the k-th largest value, as a bound: the largest t with count(key >= t) >= k in the bits that keys of
+// the type differ in (the lowest 16 of a bf16 value's are alike, 13 of an fp16 value's).  Keys below -inf's
+// are those of NaN, which nothing exceeds: where the k-th largest is -inf, t is 0.
 template <int DT, int T, int C>
 __device__ __forceinline__ uint32_t kth_key(const Row<DT, T, C>& x, int k, float* buf) {
+  constexpr int LAST = DT == ops::kDtBF16 ? 16 : DT == ops::kDtFP16 ? 13 : 0;
   uint32_t t = 0u;
-  for (int bit = 31; bit >= 0; --bit) {
+  for (int bit = 31; bit >= LAST; --bit) {
     const uint32_t cand = t | (1u << bit);
-    float n = 0.f;
-    x.each([&](float v, int) { n += v == v && sample_key(v + 0.f) >= cand ? 1.f : 0.f; });
-    if (reduce_all<T, false>(n, buf) >= (float)k) t = cand;
+    const float c = sample_unkey(cand);
+    int n = 0;
+    x.each([&](float v, int) { n += v >= c ? 1 : 0; });
+    if (reduce_all<T, false>((float)n, buf) >= (float)k) t = cand;
   }
   return t;
 }
@@ -308,17 +316,10 @@ __device__ __forceinline__ RowTop row_top(const void* base, int64_t row, int V, 
     return r;
   }
   // more values than the list holds: with k <= T the bound may lie below the k-th largest
-  if (k < V && k <= T) {
-    Row<DT, T, C> again;  // not kept in registers until here
-    asm volatile("" : "+s"(base));
-    again.load(base, row, V);
-    r.kth = max(r.kth, min(kth_key(again, k, s.buf), sample_key(__FLT_MAX__)));
-  }
+  if (k < V && k <= T) r.kth = max(r.kth, min(kth_key(x, k, s.buf), sample_key(__FLT_MAX__)));
+  const float least = sample_unkey(r.kth);
   float sum = 0.f;
-  for (int i = tid; i < V; i += T) {
-    const float v = load_logit<DT>(base, row + i);
-    if (sample_key(v) >= r.kth) sum += expf(v - r.max);
-  }
+  x.each([&](float v, int) { sum += v >= least ? expf(fminf(v, __FLT_MAX__) - r.max) : 0.f; });
   r.sum = reduce_all<T, false>(sum, s.buf);
   return r;
 }
@@ -349,7 +350,7 @@ struct WalkLds {
   int64_t tokens[kTreeNodes];
   float uniform[kTreeNodes];
   float logit[2][kTreeNodes];  // of a node's token in its parent's rows
-  float sums[kTreeNodes];      // W of p before each rejection,
+  float sums[kTreeNodes];      // 1 / sum of p before each rejection,
   int64_t gone[kTreeNodes];    // and the rejected tokens
   float buf[T / 64];
   unsigned long long best[T / 64];
@@ -399,76 +400,105 @@ __global__ __launch_bounds__(T) void verify_walk_kernel(VerifyParams p) {
       tp = row_top<DT, T, C>(p.rows[0], xat, p.V, p.k, s.row);
     }
     const u32x2* list = p.list + ((int64_t)b * p.ahead + here) * kVerifyList;
-    const int n = tp.listed ? tp.listed : p.V;
-    float W = tp.sum;
+    const int n = tp.listed;
+    double W = tp.sum, whole = W;  // p's sum, and the last that a pass over its words gave
     int gone = 0;  // rejections that changed p
     // the weight of a word (unnormalised, sum W): its kept exponential, after the rejections so far
     auto weight = [&](float w, float q, int64_t word) {
       for (int j = 0; j < gone; ++j)
-        w = DRAFT ? fmaxf(w * (1.f / s.sums[j]) - q, 0.f) : word == s.gone[j] ? 0.f : w;
+        w = DRAFT ? fmaxf(w * s.sums[j] - q, 0.f) : word == s.gone[j] ? 0.f : w;
       return w;
     };
-    // a word of the node: its index, its kept exponential (0: none) and the drafter's probability
+    // an entry of the node's list: the word, its kept exponential (0: none) and the drafter's probability
     struct Entry {
       int word;
       float w, q;
     };
     const bool asks = kids != 0;
+    const float qinv = DRAFT && asks ? 1.f / tq.sum : 0.f;
     auto entry = [&](int i) {
-      Entry e{i, 0.f, 0.f};
+      Entry e{0, 0.f, 0.f};
       if (i >= n) return e;
-      if (tp.listed) {
-        const u32x2 x = ready ? list[i] : u32x2{s.row.key[i], (uint32_t)s.row.idx[i]};
-        e.word = (int)x[1];
-        e.w = x[0] >= tp.kth ? expf(sample_unkey(x[0]) - tp.max) : 0.f;
-      } else {
-        e.w = kept(load_logit<DT>(p.rows[0], xat + i), tp);
-      }
+      const u32x2 x = ready ? list[i] : u32x2{s.row.key[i], (uint32_t)s.row.idx[i]};
+      e.word = (int)x[1];
+      e.w = x[0] >= tp.kth ? expf(sample_unkey(x[0]) - tp.max) : 0.f;
       if constexpr (DRAFT)
-        if (asks && e.w > 0.f) e.q = kept(load_logit<DT>(p.rows[1], yat + e.word), tq) * (1.f / tq.sum);
+        if (asks && e.w > 0.f) e.q = kept(load_logit<DT>(p.rows[1], yat + e.word), tq) * qinv;
       return e;
     };
-    // f(weight, q, word) over the words of this thread.  Its first is loaded once a node, when a rejection or
-    // the draw first needs it: lists are mostly shorter than the workgroup.
+    // f(weight, q, word) over the words of this thread.  Its first entry is loaded once a node, when a rejection
+    // or the draw first needs it: lists are mostly shorter than the workgroup.  Without a list, 8 words a load.
     Entry own;
     bool loaded = false;
     auto each = [&](auto f) {
-      if (!loaded) own = entry(tid);
-      loaded = true;
-      if (own.w > 0.f) f(weight(own.w, own.q, own.word), own.q, own.word);
-      for (int i = tid + T; i < n; i += T) {
-        const Entry e = entry(i);
-        if (e.w > 0.f) f(weight(e.w, e.q, e.word), e.q, e.word);
+      if (n) {
+        if (!loaded) own = entry(tid);
+        loaded = true;
+        if (own.w > 0.f) f(weight(own.w, own.q, own.word), own.q, own.word);
+        for (int i = tid + T; i < n; i += T) {
+          const Entry e = entry(i);
+          if (e.w > 0.f) f(weight(e.w, e.q, e.word), e.q, e.word);
+        }
+        return;
+      }
+      for (int i = 8 * tid; i < p.V; i += 8 * T) {
+        float x[8], y[8] = {};
+        const int m = p.V - i;
+        if (m >= 8) {
+          const auto xr = ops::load8_any<DT>(p.rows[0], xat + i);
+          if constexpr (DRAFT)
+            if (asks) ops::IO<DT>::unpack(ops::load8_any<DT>(p.rows[1], yat + i), y);
+          ops::IO<DT>::unpack(xr, x);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] = e < m ? ops::IO<DT>::load1(p.rows[0], xat + i + e) : -INFINITY;
+            if constexpr (DRAFT)
+              if (asks && e < m) y[e] = ops::IO<DT>::load1(p.rows[1], yat + i + e);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float w = e < m ? kept(as_logit(x[e]), tp) : 0.f;
+          if (!(w > 0.f)) continue;
+          float q = 0.f;
+          if constexpr (DRAFT)
+            if (asks) q = kept(as_logit(y[e]), tq) * qinv;
+          f(weight(w, q, i + e), q, i + e);
+        }
       }
     };
     int next = -1;
     while (kids) {
       const int c = __builtin_ctzll(kids);
       const int64_t x = s.tokens[c];
-      const float q = DRAFT ? kept(s.logit[1][c], tq) * (1.f / tq.sum) : 1.f;
-      const float px = weight(kept(s.logit[0][c], tp), q, x) * (1.f / W);
-      if (s.uniform[c] * q < px) {
+      const float q = DRAFT ? kept(s.logit[1][c], tq) * qinv : 1.f;
+      const float inv = 1.f / (float)W, wx = weight(kept(s.logit[0][c], tp), q, x);
+      if (s.uniform[c] * q < wx * inv) {
         next = c;
         break;
       }
-      float sum = 0.f;
-      const float inv = 1.f / W;
-      each([&](float w, float qw, int word) { sum += DRAFT ? fmaxf(w * inv - qw, 0.f) : word == x ? 0.f : w; });
-      sum = reduce_all<T, false>(sum, s.buf);
-      if (sum > 0.f) {
+      double left = W - wx;
+      // p loses x alone: its sum less x's weight, while that takes no more than half of what was added up
+      if (DRAFT || left < 0.5 * whole) {
+        float sum = 0.f;
+        each([&](float w, float qw, int word) { sum += DRAFT ? fmaxf(w * inv - qw, 0.f) : word == x ? 0.f : w; });
+        left = whole = reduce_all<T, false>(sum, s.buf);
+      }
+      if (left > 0.) {
         if (tid == 0) {
-          s.sums[gone] = W;
+          s.sums[gone] = inv;
           s.gone[gone] = x;
         }
         ++gone;
-        W = sum;
+        W = left;
         __syncthreads();
       }
       kids &= kids - 1;
     }
     here = next;
     if (next >= 0) continue;
-    const float inv = 1.f / W;
+    const float inv = 1.f / (float)W;
     const float* noise = p.noise + b * p.ldn;
     unsigned long long best = 0ull;
     each([&](float w, float, int word) {
