@@ -54,18 +54,20 @@ __device__ __forceinline__ float block_reduce_256(float v, float* buf) {
 
 constexpr int kDistillPer = kDistillEntries / 256;  // entries of a thread
 
+template <int PER>
 struct Entries {
-  int64_t idx[kDistillPer];  // -1 where there is no entry
-  float p[kDistillPer], logp[kDistillPer];
+  int64_t idx[PER];  // -1 where there is no entry
+  float p[PER], logp[PER];
   bool any;
 };
 
 // The row's entries and their probabilities, entry threadIdx.x + 256 j at slot j.
-__device__ __forceinline__ Entries load_entries(const DistillParams& a, int64_t row, float* buf) {
-  Entries e;
+template <int PER>
+__device__ __forceinline__ Entries<PER> load_entries(const DistillParams& a, int64_t row, float* buf) {
+  Entries<PER> e;
   float m = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < kDistillPer; ++j) {
+  for (int j = 0; j < PER; ++j) {
     const int i = threadIdx.x + 256 * j;
     e.idx[j] = -1;
     e.logp[j] = -INFINITY;
@@ -80,7 +82,7 @@ __device__ __forceinline__ Entries load_entries(const DistillParams& a, int64_t 
   // NaN logits: fmaxf passes over them, the sum does not
   float sum = 0.f;
 #pragma unroll
-  for (int j = 0; j < kDistillPer; ++j) {
+  for (int j = 0; j < PER; ++j) {
     e.p[j] = e.idx[j] < 0 ? 0.f : expf(e.logp[j] - m);
     sum += e.p[j];
   }
@@ -88,7 +90,7 @@ __device__ __forceinline__ Entries load_entries(const DistillParams& a, int64_t 
   e.any = !(sum == 0.f);
   const float inv = 1.f / sum, off = m + logf(sum);
 #pragma unroll
-  for (int j = 0; j < kDistillPer; ++j) {
+  for (int j = 0; j < PER; ++j) {
     e.p[j] = e.idx[j] < 0 ? 0.f : e.p[j] * inv;  // also where a NaN among the entries makes inv one
     e.logp[j] -= off;
   }
@@ -101,7 +103,7 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams a) {
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
   const int64_t base = row * a.ldx;
-  const Entries e = load_entries(a, row, buf);
+  const Entries<kDistillPer> e = load_entries<kDistillPer>(a, row, buf);
   if (!e.any) {
     if (tid == 0) *reinterpret_cast<f32x4*>(a.row + 4 * row) = f32x4{0.f, 0.f, 1.f, 0.f};
     return;
@@ -189,12 +191,28 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(float* row, int64_t r
   }
 }
 
+// Entries of one index share the gradient of its column: q minus every p of that index, which each of them
+// writes.  Up to kDistillFew entries every thread looks through all of them for its own.  MANY: a bitmap of hashed
+// indexes first tells which could have another (a few in a hundred at 1024 entries), and a wave looks for each of those.
+// 8192 rows of 16384 bf16 logits: 64 entries 102 us, 65 of them 98, 256 145 (160 without the bitmap), 1024 182 (1099).
+constexpr int kDistillFew = 64;
+constexpr int kDistillBits = 32768;
+
+template <bool MANY>
+struct DistillLds {
+  float buf[4];
+  int idx[MANY ? kDistillEntries : kDistillFew];  // -1: none
+  float prob[MANY ? kDistillEntries : kDistillFew];
+  uint32_t seen[MANY ? kDistillBits / 32 : 1], twice[MANY ? kDistillBits / 32 : 1];
+  uint16_t list[MANY ? kDistillEntries : 1];  // entries that could have another
+  int count;
+};
+
 // PAST: the gradient goes past the caches.
-template <int DT, bool PAST>
+template <int DT, bool PAST, bool MANY>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
-  __shared__ float buf[4];
-  __shared__ int64_t idx[kDistillEntries];
-  __shared__ float prob[kDistillEntries];
+  constexpr int PER = MANY ? kDistillPer : 1;  // entries of a thread
+  __shared__ DistillLds<MANY> lds;
   const int64_t row = a.rows - 1 - blockIdx.x;  // the rows that the forward read last first: some are still in a cache
   const int tid = threadIdx.x;
   const int64_t base = row * a.ldx, out = row * a.V;
@@ -206,14 +224,20 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
     if (tid < a.V - 8 * nvec) ops::IO<DT>::store1(a.dx, out + 8 * nvec + tid, 0.f);
     return;
   }
-  const Entries e = load_entries(a, row, buf);
+  const Entries<PER> e = load_entries<PER>(a, row, lds.buf);
   bool bad = false;
 #pragma unroll
-  for (int j = 0; j < kDistillPer; ++j) {
+  for (int j = 0; j < PER; ++j) {
     const int i = tid + 256 * j;
-    idx[i] = e.idx[j];
-    prob[i] = e.p[j];
+    if (MANY || i < kDistillFew) {
+      lds.idx[i] = e.idx[j] < a.V ? (int)e.idx[j] : -1;
+      lds.prob[i] = e.p[j];
+    }
     bad |= e.p[j] != 0.f && e.idx[j] >= a.V;
+  }
+  if constexpr (MANY) {
+    for (int i = tid; i < kDistillBits / 32; i += 256) lds.seen[i] = lds.twice[i] = 0u;
+    if (tid == 0) lds.count = 0;
   }
   const float c2 = a.inv_t * kLog2e, M = r[1], inv = 1.f / r[2];
   float scale = *a.grad / (a.row[4 * a.rows] * a.inv_t);
@@ -237,16 +261,44 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
     const int i = 8 * nvec + tid;
     ops::IO<DT>::store1(a.dx, out + i, exp2_fast((ops::IO<DT>::load1(a.x, base + i) - M) * c2) * qs);
   }
-  // then the entries' columns, once more and whole: q minus every p of that index (entries of
-  // one index write one value); the barrier puts these stores behind the others
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < kDistillPer; ++j) {
-    if (e.idx[j] < 0 || e.idx[j] >= a.V) continue;
+  // then the entries' columns, once more and whole; the barrier puts these stores behind the others
+  auto column = [&](int v, float P) {
+    const float q = exp2_fast((ops::IO<DT>::load1(a.x, base + v) - M) * c2) * inv;
+    ops::IO<DT>::store1(a.dx, out + v, (q - P) * scale);
+  };
+  if constexpr (!MANY) {
+    __syncthreads();
+    if (e.idx[0] < 0 || e.idx[0] >= a.V) return;
     float P = 0.f;
-    for (int i = 0; i < a.K; ++i) P += idx[i] == e.idx[j] ? prob[i] : 0.f;
-    const float q = exp2_fast((ops::IO<DT>::load1(a.x, base + e.idx[j]) - M) * c2) * inv;
-    ops::IO<DT>::store1(a.dx, out + e.idx[j], (q - P) * scale);
+    for (int i = 0; i < a.K; ++i) P += lds.idx[i] == (int)e.idx[0] ? lds.prob[i] : 0.f;
+    column((int)e.idx[0], P);
+  } else {
+    auto bit = [](int v) { return (uint32_t)v * 2654435761u >> 17; };
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int v = lds.idx[tid + 256 * j];
+      if (v < 0) continue;
+      const uint32_t h = bit(v), one = 1u << (h & 31);
+      if (atomicOr(&lds.seen[h >> 5], one) & one) atomicOr(&lds.twice[h >> 5], one);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int v = lds.idx[tid + 256 * j];
+      if (v < 0) continue;
+      const uint32_t h = bit(v);
+      if (lds.twice[h >> 5] >> (h & 31) & 1u) lds.list[atomicAdd(&lds.count, 1)] = (uint16_t)(tid + 256 * j);
+      else column(v, e.p[j]);
+    }
+    __syncthreads();
+    const int n = lds.count, lane = tid & 63;
+    for (int k = tid >> 6; k < n; k += 4) {  // in any order: an entry's sum is over all of them in theirs
+      const int v = lds.idx[lds.list[k]];
+      float P = 0.f;
+      for (int i = lane; i < a.K; i += 64) P += lds.idx[i] == v ? lds.prob[i] : 0.f;
+      P = wave_reduce<0, false>(P);
+      if (lane == 0) column(v, P);
+    }
   }
 }
 
