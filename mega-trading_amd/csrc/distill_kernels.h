@@ -191,20 +191,24 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(float* row, int64_t r
   }
 }
 
-// Entries of one index share the gradient of its column: q minus every p of that index, which each of them
-// writes.  Up to kDistillFew entries every thread looks through all of them for its own.  MANY: a bitmap of hashed
-// indexes first tells which could have another (a few in a hundred at 1024 entries), and a wave looks for each of those.
-// 8192 rows of 16384 bf16 logits: 64 entries 102 us, 65 of them 98, 256 145 (160 without the bitmap), 1024 182 (1099).
+// A gradient is stored once, whole: a column that an entry names takes its P on the way.  So the entries
+// are laid out first: those of one index share the sum of their p, in their order, and the first of them goes into
+// a table by the column's group of 8.  Up to kDistillFew entries, one a thread, look through all of them for their
+// own; MANY: a bitmap of hashed indexes first tells which could have another (a few in a hundred at 1024 entries), and
+// a wave looks for each of those.  (Stored again after the others instead, the named columns cost 65 of 425 us at
+// 32768 rows of 16384 bf16 logits with 64 entries: parts of lines that had left the caches.)
 constexpr int kDistillFew = 64;
-constexpr int kDistillBits = 32768;
+constexpr int kDistillTable = 2048;
+constexpr int kDistillBits = kDistillTable / 2 * 32;  // both bitmaps lie where the table will be
 
-template <bool MANY>
+template <int ENT>
 struct DistillLds {
   float buf[4];
-  int idx[MANY ? kDistillEntries : kDistillFew];  // -1: none
-  float prob[MANY ? kDistillEntries : kDistillFew];
-  uint32_t seen[MANY ? kDistillBits / 32 : 1], twice[MANY ? kDistillBits / 32 : 1];
-  uint16_t list[MANY ? kDistillEntries : 1];  // entries that could have another
+  uint32_t table[kDistillTable];  // the first entry of a group's, plus 1
+  int idx[ENT];                   // -1: none
+  float prob[ENT], sum[ENT];      // p, and of all entries of the index
+  uint16_t next[ENT];             // entry of the group, plus 1
+  uint16_t list[ENT];             // MANY: entries that could have another
   int count;
 };
 
@@ -212,7 +216,7 @@ struct DistillLds {
 template <int DT, bool PAST, bool MANY>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
   constexpr int PER = MANY ? kDistillPer : 1;  // entries of a thread
-  __shared__ DistillLds<MANY> lds;
+  __shared__ DistillLds<MANY ? kDistillEntries : kDistillFew> lds;
   const int64_t row = a.rows - 1 - blockIdx.x;  // the rows that the forward read last first: some are still in a cache
   const int tid = threadIdx.x;
   const int64_t base = row * a.ldx, out = row * a.V;
@@ -226,79 +230,113 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
   }
   const Entries<PER> e = load_entries<PER>(a, row, lds.buf);
   bool bad = false;
+  int idx[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int i = tid + 256 * j;
+    idx[j] = e.idx[j] < a.V ? (int)e.idx[j] : -1;
     if (MANY || i < kDistillFew) {
-      lds.idx[i] = e.idx[j] < a.V ? (int)e.idx[j] : -1;
-      lds.prob[i] = e.p[j];
+      lds.idx[i] = idx[j];
+      lds.prob[i] = lds.sum[i] = e.p[j];
     }
     bad |= e.p[j] != 0.f && e.idx[j] >= a.V;
   }
-  if constexpr (MANY) {
-    for (int i = tid; i < kDistillBits / 32; i += 256) lds.seen[i] = lds.twice[i] = 0u;
-    if (tid == 0) lds.count = 0;
-  }
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < kDistillTable / 256; ++i) lds.table[tid + 256 * i] = 0u;
+  };
+  clear();
+  if (tid == 0) lds.count = 0;
   const float c2 = a.inv_t * kLog2e, M = r[1], inv = 1.f / r[2];
   float scale = *a.grad / (a.row[4 * a.rows] * a.inv_t);
   if (__syncthreads_or(bad)) scale = __builtin_nanf("");
   const float qs = inv * scale;
+  auto insert = [&](int i, int v) { lds.next[i] = (uint16_t)atomicExch(&lds.table[v / 8 % kDistillTable], (uint32_t)i + 1u); };
+  if constexpr (!MANY) {
+    if (idx[0] >= 0) {
+      float P = 0.f;
+      bool first = true;
+      for (int i = 0; i < a.K; ++i) {
+        const bool same = lds.idx[i] == idx[0];
+        P += same ? lds.prob[i] : 0.f;
+        first &= !same || i >= tid;
+      }
+      if (first) {
+        lds.sum[tid] = P;
+        insert(tid, idx[0]);
+      }
+    }
+  } else {
+    uint32_t *seen = lds.table, *twice = lds.table + kDistillBits / 32;
+    auto bit = [](int v) { return (uint32_t)v * 2654435761u >> 17; };
+    static_assert(kDistillBits == 1 << 15, "the hash's bits");
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (idx[j] < 0) continue;
+      const uint32_t h = bit(idx[j]), one = 1u << (h & 31);
+      if (atomicOr(&seen[h >> 5], one) & one) atomicOr(&twice[h >> 5], one);
+    }
+    __syncthreads();
+    bool alone[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const uint32_t h = bit(idx[j]);
+      alone[j] = idx[j] >= 0 && !(twice[h >> 5] >> (h & 31) & 1u);
+      if (idx[j] >= 0 && !alone[j]) lds.list[atomicAdd(&lds.count, 1)] = (uint16_t)(tid + 256 * j);
+    }
+    __syncthreads();
+    clear();
+    const int n = lds.count, lane = tid & 63;
+    for (int k = tid >> 6; k < n; k += 4) {  // in any order: an entry's sum is over all of them in theirs
+      const int at = lds.list[k], v = lds.idx[at];
+      float P = 0.f;
+      bool later = false;  // one of the index comes before
+      for (int i = lane; i < a.K; i += 64) {
+        const bool same = lds.idx[i] == v;
+        P += same ? lds.prob[i] : 0.f;
+        later |= same && i < at;
+      }
+      P = wave_reduce<0, false>(P);
+      const bool any = __ballot(later) != 0;
+      if (lane == 0) {
+        lds.sum[at] = P;
+        lds.next[at] = any;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (idx[j] >= 0 && (alone[j] || !lds.next[tid + 256 * j])) insert(tid + 256 * j, idx[j]);
+  }
+  __syncthreads();
   for (int c0 = tid; c0 < nvec; c0 += 256 * kDistillAhead) {
     typename ops::IO<DT>::Raw r[kDistillAhead];
 #pragma unroll
     for (int i = 0; i < kDistillAhead; ++i) r[i] = ops::load8_any<DT>(a.x, base + 8 * min(c0 + 256 * i, nvec - 1));
 #pragma unroll
     for (int i = 0; i < kDistillAhead; ++i) {
-      if (c0 + 256 * i >= nvec) continue;
+      const int c = c0 + 256 * i;
+      if (c >= nvec) continue;
       float v[8];
       ops::IO<DT>::unpack(r[i], v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = exp2_fast((v[j] - M) * c2) * qs;
-      ops::store8_any<DT, PAST>(a.dx, out + 8 * (c0 + 256 * i), v);
+      for (uint32_t h = lds.table[c % kDistillTable]; h; h = lds.next[h - 1]) {
+        const int at = lds.idx[h - 1];
+        if (at / 8 != c) continue;
+        const float P = lds.sum[h - 1] * scale;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] -= at % 8 == j ? P : 0.f;
+      }
+      ops::store8_any<DT, PAST>(a.dx, out + 8 * c, v);
     }
   }
   if (tid < a.V - 8 * nvec) {
     const int i = 8 * nvec + tid;
-    ops::IO<DT>::store1(a.dx, out + i, exp2_fast((ops::IO<DT>::load1(a.x, base + i) - M) * c2) * qs);
-  }
-  // then the entries' columns, once more and whole; the barrier puts these stores behind the others
-  auto column = [&](int v, float P) {
-    const float q = exp2_fast((ops::IO<DT>::load1(a.x, base + v) - M) * c2) * inv;
-    ops::IO<DT>::store1(a.dx, out + v, (q - P) * scale);
-  };
-  if constexpr (!MANY) {
-    __syncthreads();
-    if (e.idx[0] < 0 || e.idx[0] >= a.V) return;
-    float P = 0.f;
-    for (int i = 0; i < a.K; ++i) P += lds.idx[i] == (int)e.idx[0] ? lds.prob[i] : 0.f;
-    column((int)e.idx[0], P);
-  } else {
-    auto bit = [](int v) { return (uint32_t)v * 2654435761u >> 17; };
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int v = lds.idx[tid + 256 * j];
-      if (v < 0) continue;
-      const uint32_t h = bit(v), one = 1u << (h & 31);
-      if (atomicOr(&lds.seen[h >> 5], one) & one) atomicOr(&lds.twice[h >> 5], one);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int v = lds.idx[tid + 256 * j];
-      if (v < 0) continue;
-      const uint32_t h = bit(v);
-      if (lds.twice[h >> 5] >> (h & 31) & 1u) lds.list[atomicAdd(&lds.count, 1)] = (uint16_t)(tid + 256 * j);
-      else column(v, e.p[j]);
-    }
-    __syncthreads();
-    const int n = lds.count, lane = tid & 63;
-    for (int k = tid >> 6; k < n; k += 4) {  // in any order: an entry's sum is over all of them in theirs
-      const int v = lds.idx[lds.list[k]];
-      float P = 0.f;
-      for (int i = lane; i < a.K; i += 64) P += lds.idx[i] == v ? lds.prob[i] : 0.f;
-      P = wave_reduce<0, false>(P);
-      if (lane == 0) column(v, P);
-    }
+    float v = exp2_fast((ops::IO<DT>::load1(a.x, base + i) - M) * c2) * qs;
+    for (uint32_t h = lds.table[nvec % kDistillTable]; h; h = lds.next[h - 1])
+      if (lds.idx[h - 1] == i) v -= lds.sum[h - 1] * scale;
+    ops::IO<DT>::store1(a.dx, out + i, v);
   }
 }
 
