@@ -15,8 +15,8 @@
 // address.  The backward starts with the rows that the forward read last: part of them
 // is still in the 256 MB cache in front of the memory (688 -> 670 us for the step).
 //
-// 32768 rows of 16384 bf16 logits, 64 entries: forward 178 us (6.0 TB/s), its sum 10,
-// backward 426 (5.0 TB/s read and written, what a large copy reaches).
+// 32768 rows of 16384 bf16 logits, 64 entries: forward 178 to 198 us (5.4 to 6.0 TB/s), its
+// sum 11, backward 354 to 373 (5.8 to 6.1 TB/s read and written).
 #pragma once
 
 #include "storage.h"
@@ -54,20 +54,18 @@ __device__ __forceinline__ float block_reduce_256(float v, float* buf) {
 
 constexpr int kDistillPer = kDistillEntries / 256;  // entries of a thread
 
-template <int PER>
 struct Entries {
-  int64_t idx[PER];  // -1 where there is no entry
-  float p[PER], logp[PER];
+  int64_t idx[kDistillPer];  // -1 where there is no entry
+  float p[kDistillPer], logp[kDistillPer];
   bool any;
 };
 
 // The row's entries and their probabilities, entry threadIdx.x + 256 j at slot j.
-template <int PER>
-__device__ __forceinline__ Entries<PER> load_entries(const DistillParams& a, int64_t row, float* buf) {
-  Entries<PER> e;
+__device__ __forceinline__ Entries load_entries(const DistillParams& a, int64_t row, float* buf) {
+  Entries e;
   float m = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
+  for (int j = 0; j < kDistillPer; ++j) {
     const int i = threadIdx.x + 256 * j;
     e.idx[j] = -1;
     e.logp[j] = -INFINITY;
@@ -82,7 +80,7 @@ __device__ __forceinline__ Entries<PER> load_entries(const DistillParams& a, int
   // NaN logits: fmaxf passes over them, the sum does not
   float sum = 0.f;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
+  for (int j = 0; j < kDistillPer; ++j) {
     e.p[j] = e.idx[j] < 0 ? 0.f : expf(e.logp[j] - m);
     sum += e.p[j];
   }
@@ -90,7 +88,7 @@ __device__ __forceinline__ Entries<PER> load_entries(const DistillParams& a, int
   e.any = !(sum == 0.f);
   const float inv = 1.f / sum, off = m + logf(sum);
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
+  for (int j = 0; j < kDistillPer; ++j) {
     e.p[j] = e.idx[j] < 0 ? 0.f : e.p[j] * inv;  // also where a NaN among the entries makes inv one
     e.logp[j] -= off;
   }
@@ -103,7 +101,7 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams a) {
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
   const int64_t base = row * a.ldx;
-  const Entries<kDistillPer> e = load_entries<kDistillPer>(a, row, buf);
+  const Entries e = load_entries(a, row, buf);
   if (!e.any) {
     if (tid == 0) *reinterpret_cast<f32x4*>(a.row + 4 * row) = f32x4{0.f, 0.f, 1.f, 0.f};
     return;
@@ -193,30 +191,27 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(float* row, int64_t r
 
 // A gradient is stored once, whole: a column that an entry names takes its P on the way.  So the entries
 // are laid out first: those of one index share the sum of their p, in their order, and the first of them goes into
-// a table by the column's group of 8.  Up to kDistillFew entries, one a thread, look through all of them for their
-// own; MANY: a bitmap of hashed indexes first tells which could have another (a few in a hundred at 1024 entries), and
-// a wave looks for each of those.  (Stored again after the others instead, the named columns cost 65 of 425 us at
-// 32768 rows of 16384 bf16 logits with 64 entries: parts of lines that had left the caches.)
-constexpr int kDistillFew = 64;
+// a table by the column's group of 8.  A bitmap of hashed indexes tells which could have another (a few in a hundred at
+// 1024 entries), and a wave looks for each of those (8192 rows of 16384 bf16 logits: 84 us with 64 entries, where every
+// thread looking through all of them for its own takes 93; 102 with 1024, 1099 so).  Stored again after the others
+// instead, the named columns cost 65 of 425 us at 32768 rows with 64 entries: parts of lines that had left the caches.
 constexpr int kDistillTable = 2048;
 constexpr int kDistillBits = kDistillTable / 2 * 32;  // both bitmaps lie where the table will be
 
-template <int ENT>
 struct DistillLds {
   float buf[4];
   uint32_t table[kDistillTable];  // the first entry of a group's, plus 1
-  int idx[ENT];                   // -1: none
-  float prob[ENT], sum[ENT];      // p, and of all entries of the index
-  uint16_t next[ENT];             // entry of the group, plus 1
-  uint16_t list[ENT];             // MANY: entries that could have another
+  int idx[kDistillEntries];        // -1: none
+  float prob[kDistillEntries], sum[kDistillEntries];      // p, and of all entries of the index
+  uint16_t next[kDistillEntries];  // entry of the group, plus 1
+  uint16_t list[kDistillEntries];  // entries that could have another
   int count;
 };
 
 // PAST: the gradient goes past the caches.
-template <int DT, bool PAST, bool MANY>
+template <int DT, bool PAST>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
-  constexpr int PER = MANY ? kDistillPer : 1;  // entries of a thread
-  __shared__ DistillLds<MANY ? kDistillEntries : kDistillFew> lds;
+  __shared__ DistillLds lds;
   const int64_t row = a.rows - 1 - blockIdx.x;  // the rows that the forward read last first: some are still in a cache
   const int tid = threadIdx.x;
   const int64_t base = row * a.ldx, out = row * a.V;
@@ -228,17 +223,15 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
     if (tid < a.V - 8 * nvec) ops::IO<DT>::store1(a.dx, out + 8 * nvec + tid, 0.f);
     return;
   }
-  const Entries<PER> e = load_entries<PER>(a, row, lds.buf);
+  const Entries e = load_entries(a, row, lds.buf);
   bool bad = false;
-  int idx[PER];
+  int idx[kDistillPer];
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
+  for (int j = 0; j < kDistillPer; ++j) {
     const int i = tid + 256 * j;
     idx[j] = e.idx[j] < a.V ? (int)e.idx[j] : -1;
-    if (MANY || i < kDistillFew) {
-      lds.idx[i] = idx[j];
-      lds.prob[i] = lds.sum[i] = e.p[j];
-    }
+    lds.idx[i] = idx[j];
+    lds.prob[i] = lds.sum[i] = e.p[j];
     bad |= e.p[j] != 0.f && e.idx[j] >= a.V;
   }
   auto clear = [&]() {
@@ -252,62 +245,46 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
   if (__syncthreads_or(bad)) scale = __builtin_nanf("");
   const float qs = inv * scale;
   auto insert = [&](int i, int v) { lds.next[i] = (uint16_t)atomicExch(&lds.table[v / 8 % kDistillTable], (uint32_t)i + 1u); };
-  if constexpr (!MANY) {
-    if (idx[0] >= 0) {
-      float P = 0.f;
-      bool first = true;
-      for (int i = 0; i < a.K; ++i) {
-        const bool same = lds.idx[i] == idx[0];
-        P += same ? lds.prob[i] : 0.f;
-        first &= !same || i >= tid;
-      }
-      if (first) {
-        lds.sum[tid] = P;
-        insert(tid, idx[0]);
-      }
-    }
-  } else {
-    uint32_t *seen = lds.table, *twice = lds.table + kDistillBits / 32;
-    auto bit = [](int v) { return (uint32_t)v * 2654435761u >> 17; };
-    static_assert(kDistillBits == 1 << 15, "the hash's bits");
+  uint32_t *seen = lds.table, *twice = lds.table + kDistillBits / 32;
+  auto bit = [](int v) { return (uint32_t)v * 2654435761u >> 17; };
+  static_assert(kDistillBits == 1 << 15, "the hash's bits");
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      if (idx[j] < 0) continue;
-      const uint32_t h = bit(idx[j]), one = 1u << (h & 31);
-      if (atomicOr(&seen[h >> 5], one) & one) atomicOr(&twice[h >> 5], one);
-    }
-    __syncthreads();
-    bool alone[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const uint32_t h = bit(idx[j]);
-      alone[j] = idx[j] >= 0 && !(twice[h >> 5] >> (h & 31) & 1u);
-      if (idx[j] >= 0 && !alone[j]) lds.list[atomicAdd(&lds.count, 1)] = (uint16_t)(tid + 256 * j);
-    }
-    __syncthreads();
-    clear();
-    const int n = lds.count, lane = tid & 63;
-    for (int k = tid >> 6; k < n; k += 4) {  // in any order: an entry's sum is over all of them in theirs
-      const int at = lds.list[k], v = lds.idx[at];
-      float P = 0.f;
-      bool later = false;  // one of the index comes before
-      for (int i = lane; i < a.K; i += 64) {
-        const bool same = lds.idx[i] == v;
-        P += same ? lds.prob[i] : 0.f;
-        later |= same && i < at;
-      }
-      P = wave_reduce<0, false>(P);
-      const bool any = __ballot(later) != 0;
-      if (lane == 0) {
-        lds.sum[at] = P;
-        lds.next[at] = any;
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (idx[j] >= 0 && (alone[j] || !lds.next[tid + 256 * j])) insert(tid + 256 * j, idx[j]);
+  for (int j = 0; j < kDistillPer; ++j) {
+    if (idx[j] < 0) continue;
+    const uint32_t h = bit(idx[j]), one = 1u << (h & 31);
+    if (atomicOr(&seen[h >> 5], one) & one) atomicOr(&twice[h >> 5], one);
   }
+  __syncthreads();
+  bool alone[kDistillPer];
+#pragma unroll
+  for (int j = 0; j < kDistillPer; ++j) {
+    const uint32_t h = bit(idx[j]);
+    alone[j] = idx[j] >= 0 && !(twice[h >> 5] >> (h & 31) & 1u);
+    if (idx[j] >= 0 && !alone[j]) lds.list[atomicAdd(&lds.count, 1)] = (uint16_t)(tid + 256 * j);
+  }
+  __syncthreads();
+  clear();
+  const int n = lds.count, lane = tid & 63;
+  for (int k = tid >> 6; k < n; k += 4) {  // in any order: an entry's sum is over all of them in theirs
+    const int at = lds.list[k], v = lds.idx[at];
+    float P = 0.f;
+    bool later = false;  // one of the index comes before
+    for (int i = lane; i < a.K; i += 64) {
+      const bool same = lds.idx[i] == v;
+      P += same ? lds.prob[i] : 0.f;
+      later |= same && i < at;
+    }
+    P = wave_reduce<0, false>(P);
+    const bool any = __ballot(later) != 0;
+    if (lane == 0) {
+      lds.sum[at] = P;
+      lds.next[at] = any;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kDistillPer; ++j)
+    if (idx[j] >= 0 && (alone[j] || !lds.next[tid + 256 * j])) insert(tid + 256 * j, idx[j]);
   __syncthreads();
   for (int c0 = tid; c0 < nvec; c0 += 256 * kDistillAhead) {
     typename ops::IO<DT>::Raw r[kDistillAhead];

@@ -145,6 +145,24 @@ def test_a_logit_that_is_no_number_spoils_its_row_alone(mta, where):
     assert math.isnan(float(mta.ops.topk_distillation(x[1:2].to(DEV), y[1:2].to(DEV), i[1:2].to(DEV))))
 
 
+def test_entries_of_one_index_and_of_one_group(mta):
+    """Every entry the same index; pairs and triples of it; and indexes 16384 apart or in one group of 8 columns."""
+    vocab, top = 50001, 300
+    x, y, i = inputs(7, vocab, top, F32, 23)
+    j = torch.arange(top)
+    i[0] = 777
+    i[1] = j // 2 * 100
+    i[2] = j // 3 * 8 + 5
+    i[3] = j % 3 * 16384 + j // 3 * 3
+    i[4] = 40000 + j % 16
+    i[5] = vocab - 1 - j % 2  # the columns past the last whole group
+    i[6] = j
+    check(mta, x, y, i, temperature=2.0)
+    g = [torch.autograd.grad(mta.ops.topk_distillation(t, y.to(DEV), i.to(DEV)), t)[0]
+         for t in (x.to(DEV).requires_grad_(True) for _ in range(3))]
+    assert torch.equal(g[0], g[1]) and torch.equal(g[0], g[2])
+
+
 def test_layouts_and_types_of_the_teacher(mta):
     x, y, i = inputs(12, 101, 8, BF16, 5)
     ref = check(mta, x, y.to(BF16), i, 2.0)
