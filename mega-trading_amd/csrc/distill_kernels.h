@@ -54,18 +54,20 @@ __device__ __forceinline__ float block_reduce_256(float v, float* buf) {
 
 constexpr int kDistillPer = kDistillEntries / 256;  // entries of a thread
 
+template <int PER>
 struct Entries {
-  int64_t idx[kDistillPer];  // -1 where there is no entry
-  float p[kDistillPer], logp[kDistillPer];
+  int64_t idx[PER];  // -1 where there is no entry
+  float p[PER], logp[PER];
   bool any;
 };
 
 // The row's entries and their probabilities, entry threadIdx.x + 256 j at slot j.
-__device__ __forceinline__ Entries load_entries(const DistillParams& a, int64_t row, float* buf) {
-  Entries e;
+template <int PER>
+__device__ __forceinline__ Entries<PER> load_entries(const DistillParams& a, int64_t row, float* buf) {
+  Entries<PER> e;
   float m = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < kDistillPer; ++j) {
+  for (int j = 0; j < PER; ++j) {
     const int i = threadIdx.x + 256 * j;
     e.idx[j] = -1;
     e.logp[j] = -INFINITY;
@@ -80,7 +82,7 @@ __device__ __forceinline__ Entries load_entries(const DistillParams& a, int64_t 
   // NaN logits: fmaxf passes over them, the sum does not
   float sum = 0.f;
 #pragma unroll
-  for (int j = 0; j < kDistillPer; ++j) {
+  for (int j = 0; j < PER; ++j) {
     e.p[j] = e.idx[j] < 0 ? 0.f : expf(e.logp[j] - m);
     sum += e.p[j];
   }
@@ -88,7 +90,7 @@ __device__ __forceinline__ Entries load_entries(const DistillParams& a, int64_t 
   e.any = !(sum == 0.f);
   const float inv = 1.f / sum, off = m + logf(sum);
 #pragma unroll
-  for (int j = 0; j < kDistillPer; ++j) {
+  for (int j = 0; j < PER; ++j) {
     e.p[j] = e.idx[j] < 0 ? 0.f : e.p[j] * inv;  // also where a NaN among the entries makes inv one
     e.logp[j] -= off;
   }
@@ -97,11 +99,12 @@ __device__ __forceinline__ Entries load_entries(const DistillParams& a, int64_t 
 
 template <int DT>
 __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams a) {
+  constexpr int PER = kDistillPer;
   __shared__ float buf[4];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
   const int64_t base = row * a.ldx;
-  const Entries e = load_entries(a, row, buf);
+  const Entries<PER> e = load_entries<PER>(a, row, buf);
   if (!e.any) {
     if (tid == 0) *reinterpret_cast<f32x4*>(a.row + 4 * row) = f32x4{0.f, 0.f, 1.f, 0.f};
     return;
@@ -144,7 +147,7 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(DistillParams a) {
   const float logs = logf(s);
   float loss = 0.f;
 #pragma unroll
-  for (int j = 0; j < kDistillPer; ++j)
+  for (int j = 0; j < PER; ++j)
     if (e.idx[j] >= 0 && e.p[j] != 0.f) {
       const bool in = e.idx[j] < a.V;
       const float xi = ops::IO<DT>::load1(a.x, base + (in ? e.idx[j] : 0));
@@ -195,23 +198,28 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(float* row, int64_t r
 // 1024 entries), and a wave looks for each of those (8192 rows of 16384 bf16 logits: 84 us with 64 entries, where every
 // thread looking through all of them for its own takes 93; 102 with 1024, 1099 so).  Stored again after the others
 // instead, the named columns cost 65 of 425 us at 32768 rows with 64 entries: parts of lines that had left the caches.
-constexpr int kDistillTable = 2048;
-constexpr int kDistillBits = kDistillTable / 2 * 32;  // both bitmaps lie where the table will be
+//
+// Up to kDistillFew entries have a smaller table: less LDS to clear, and more rows on a CU (28337 rows of 663 fp32
+// logits, 6 entries: 54 us, 84 in the large one; rows of 16384 take the same time in both).
+constexpr int kDistillFew = 64;
 
+template <int ENT, int TABLE>
 struct DistillLds {
   float buf[4];
-  uint32_t table[kDistillTable];  // the first entry of a group's, plus 1
-  int idx[kDistillEntries];        // -1: none
-  float prob[kDistillEntries], sum[kDistillEntries];      // p, and of all entries of the index
-  uint16_t next[kDistillEntries];  // entry of the group, plus 1
-  uint16_t list[kDistillEntries];  // entries that could have another
+  uint32_t table[TABLE];      // the first entry of a group's, plus 1
+  int idx[ENT];               // -1: none
+  float prob[ENT], sum[ENT];  // p, and of all entries of the index
+  uint16_t next[ENT];         // entry of the group, plus 1
+  uint16_t list[ENT];         // entries that could have another
   int count;
 };
 
 // PAST: the gradient goes past the caches.
-template <int DT, bool PAST>
+template <int DT, bool PAST, int ENT>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
-  __shared__ DistillLds lds;
+  constexpr int TABLE = ENT == kDistillFew ? 256 : 2048, BITS = TABLE / 2 * 32;  // both bitmaps lie where the table will be
+  constexpr int PER = ENT > 256 ? ENT / 256 : 1;  // entries of a thread
+  __shared__ DistillLds<ENT, TABLE> lds;
   const int64_t row = a.rows - 1 - blockIdx.x;  // the rows that the forward read last first: some are still in a cache
   const int tid = threadIdx.x;
   const int64_t base = row * a.ldx, out = row * a.V;
@@ -223,20 +231,22 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
     if (tid < a.V - 8 * nvec) ops::IO<DT>::store1(a.dx, out + 8 * nvec + tid, 0.f);
     return;
   }
-  const Entries e = load_entries(a, row, lds.buf);
+  const Entries<PER> e = load_entries<PER>(a, row, lds.buf);
   bool bad = false;
-  int idx[kDistillPer];
+  int idx[PER];
 #pragma unroll
-  for (int j = 0; j < kDistillPer; ++j) {
+  for (int j = 0; j < PER; ++j) {
     const int i = tid + 256 * j;
     idx[j] = e.idx[j] < a.V ? (int)e.idx[j] : -1;
-    lds.idx[i] = idx[j];
-    lds.prob[i] = lds.sum[i] = e.p[j];
+    if (i < ENT) {
+      lds.idx[i] = idx[j];
+      lds.prob[i] = lds.sum[i] = e.p[j];
+    }
     bad |= e.p[j] != 0.f && e.idx[j] >= a.V;
   }
   auto clear = [&]() {
 #pragma unroll
-    for (int i = 0; i < kDistillTable / 256; ++i) lds.table[tid + 256 * i] = 0u;
+    for (int i = 0; i < TABLE / 256; ++i) lds.table[tid + 256 * i] = 0u;
   };
   clear();
   if (tid == 0) lds.count = 0;
@@ -244,20 +254,20 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
   float scale = *a.grad / (a.row[4 * a.rows] * a.inv_t);
   if (__syncthreads_or(bad)) scale = __builtin_nanf("");
   const float qs = inv * scale;
-  auto insert = [&](int i, int v) { lds.next[i] = (uint16_t)atomicExch(&lds.table[v / 8 % kDistillTable], (uint32_t)i + 1u); };
-  uint32_t *seen = lds.table, *twice = lds.table + kDistillBits / 32;
-  auto bit = [](int v) { return (uint32_t)v * 2654435761u >> 17; };
-  static_assert(kDistillBits == 1 << 15, "the hash's bits");
+  auto insert = [&](int i, int v) { lds.next[i] = (uint16_t)atomicExch(&lds.table[v / 8 % TABLE], (uint32_t)i + 1u); };
+  uint32_t *seen = lds.table, *twice = lds.table + BITS / 32;
+  auto bit = [](int v) { return (uint32_t)v * 2654435761u >> (ENT == kDistillFew ? 20 : 17); };
+  static_assert(BITS == (ENT == kDistillFew ? 1 << 12 : 1 << 15), "the hash's bits");
 #pragma unroll
-  for (int j = 0; j < kDistillPer; ++j) {
+  for (int j = 0; j < PER; ++j) {
     if (idx[j] < 0) continue;
     const uint32_t h = bit(idx[j]), one = 1u << (h & 31);
     if (atomicOr(&seen[h >> 5], one) & one) atomicOr(&twice[h >> 5], one);
   }
   __syncthreads();
-  bool alone[kDistillPer];
+  bool alone[PER];
 #pragma unroll
-  for (int j = 0; j < kDistillPer; ++j) {
+  for (int j = 0; j < PER; ++j) {
     const uint32_t h = bit(idx[j]);
     alone[j] = idx[j] >= 0 && !(twice[h >> 5] >> (h & 31) & 1u);
     if (idx[j] >= 0 && !alone[j]) lds.list[atomicAdd(&lds.count, 1)] = (uint16_t)(tid + 256 * j);
@@ -283,7 +293,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
   }
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < kDistillPer; ++j)
+  for (int j = 0; j < PER; ++j)
     if (idx[j] >= 0 && (alone[j] || !lds.next[tid + 256 * j])) insert(tid + 256 * j, idx[j]);
   __syncthreads();
   for (int c0 = tid; c0 < nvec; c0 += 256 * kDistillAhead) {
@@ -298,7 +308,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
       ops::IO<DT>::unpack(r[i], v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = exp2_fast((v[j] - M) * c2) * qs;
-      for (uint32_t h = lds.table[c % kDistillTable]; h; h = lds.next[h - 1]) {
+      for (uint32_t h = lds.table[c % TABLE]; h; h = lds.next[h - 1]) {
         const int at = lds.idx[h - 1];
         if (at / 8 != c) continue;
         const float P = lds.sum[h - 1] * scale;
@@ -311,7 +321,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(DistillParams a) {
   if (tid < a.V - 8 * nvec) {
     const int i = 8 * nvec + tid;
     float v = exp2_fast((ops::IO<DT>::load1(a.x, base + i) - M) * c2) * qs;
-    for (uint32_t h = lds.table[nvec % kDistillTable]; h; h = lds.next[h - 1])
+    for (uint32_t h = lds.table[nvec % TABLE]; h; h = lds.next[h - 1])
       if (lds.idx[h - 1] == i) v -= lds.sum[h - 1] * scale;
     ops::IO<DT>::store1(a.dx, out + i, v);
   }

@@ -505,12 +505,17 @@ int mt_topk_distill_bwd(const void* logits, int64_t row_stride, const float* tea
   // A gradient larger than the 256 MB cache in front of the memory cannot stay there: stored past it, it
   // leaves the logits (32768 x 16384 bf16: 355 us, and 221 for the forward of the next step; 354 + 198 past it).
   const bool past = rows * vocab * (dtype == MT_DTYPE_FP32 ? 4 : 2) > int64_t(256) << 20;
-#define MT_DISTILL_BWD(DT)                                                                        \
-  if (past) hipLaunchKernelGGL((mt::distill_bwd_kernel<DT, true>), grid, dim3(256), 0, st, p);    \
-  else hipLaunchKernelGGL((mt::distill_bwd_kernel<DT, false>), grid, dim3(256), 0, st, p)
-  if (dtype == MT_DTYPE_BF16) { MT_DISTILL_BWD(kDtBF16); }
-  else if (dtype == MT_DTYPE_FP16) { MT_DISTILL_BWD(kDtFP16); }
-  else { MT_DISTILL_BWD(kDtFP32); }
+  const bool few = entries <= mt::kDistillFew;
+#define MT_DISTILL_BWD2(DT, PAST)                                                                                  \
+  if (few) hipLaunchKernelGGL((mt::distill_bwd_kernel<DT, PAST, mt::kDistillFew>), grid, dim3(256), 0, st, p);     \
+  else hipLaunchKernelGGL((mt::distill_bwd_kernel<DT, PAST, mt::kDistillEntries>), grid, dim3(256), 0, st, p)
+#define MT_DISTILL_BWD(DT)                 \
+  if (past) { MT_DISTILL_BWD2(DT, true); } \
+  else { MT_DISTILL_BWD2(DT, false); }
+  if (dtype == MT_DTYPE_BF16) { MT_DISTILL_BWD(kDtBF16) }
+  else if (dtype == MT_DTYPE_FP16) { MT_DISTILL_BWD(kDtFP16) }
+  else { MT_DISTILL_BWD(kDtFP32) }
+#undef MT_DISTILL_BWD2
 #undef MT_DISTILL_BWD
   return launched("distillation");
 }

@@ -145,9 +145,10 @@ def test_a_logit_that_is_no_number_spoils_its_row_alone(mta, where):
     assert math.isnan(float(mta.ops.topk_distillation(x[1:2].to(DEV), y[1:2].to(DEV), i[1:2].to(DEV))))
 
 
-def test_entries_of_one_index_and_of_one_group(mta):
+@pytest.mark.parametrize("top", [64, 65, 300])
+def test_entries_of_one_index_and_of_one_group(mta, top):
     """Every entry the same index; pairs and triples of it; and indexes 16384 apart or in one group of 8 columns."""
-    vocab, top = 50001, 300
+    vocab = 50001
     x, y, i = inputs(7, vocab, top, F32, 23)
     j = torch.arange(top)
     i[0] = 777
